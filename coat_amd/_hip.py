@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get("COAT_HIP_LIB") or os.path.join(_HERE, "libcoat_hip.so
 F32, BF16, F16 = 0, 1, 2
 MAX_SLOTS, MAX_SLOT_STRIDE = 16, 32  # COAT_MAX_SLOTS, COAT_MAX_SLOT_STRIDE of include/coat_hip.h
 MAX_WORDS = MAX_SLOTS * MAX_SLOT_STRIDE
-ABI_VERSION = 5  # COAT_ABI_VERSION of include/coat_hip.h: a library built from another header is refused
+ABI_VERSION = 6  # COAT_ABI_VERSION of include/coat_hip.h: a library built from another header is refused
 E4M3, E5M2 = 0, 1
 
 _DTYPE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
@@ -74,6 +74,14 @@ SIGNATURES = {
     "coat_fp8_adamw_step": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _f, _i, _i, _i64, _i64, _vp],
     "coat_fp8_adamw_expand_step_multi": [_i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _f,
                                          _i, _i, _i, _vp],
+    "coat_layer_norm_forward": [_vp, _i64, _i, _vp, _vp, _i, _vp, _vp, _vp, _i64, _i64, _f, _vp],
+    "coat_layer_norm_partials": [_i64, _i64],
+    "coat_layer_norm_backward": [_vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i64, _i64, _vp],
+    "coat_rope_axes": [_vp, _vp, _i64, _i64, _i64, _i, _vp, _vp, _i64, _i64, _i64, _i, _i, _vp, _i64, _i64, _i64, _i, _vp, _vp, _i, _i, _i,
+                       _i, _i64, _i64, _vp],
+    "coat_grad_norm_partials": [_i, _vp],
+    "coat_grad_norm_multi": [_i, _vp, _vp, _vp, _f, _vp, _i, _vp, _vp],
+    "coat_adamw_step_multi": [_i, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp],
     "coat_fp8_adamw_step_multi": [_i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _f, _i, _i, _vp],
 }
 
@@ -129,6 +137,19 @@ def fp8(dtype):
 
 def stream(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def launch(name, device, *args, what=None):
+    """Calls entry point ``name`` with ``args`` and the current stream of ``device``, with that device current for the launch,
+    and raises on a status other than 0.  Pointers are plain integers (``Tensor.data_ptr()``) or None."""
+    fn = getattr(lib(), name)
+    if device.index is None or device.index == torch.cuda.current_device():
+        status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if status:
+        check(status, what or name)
 
 
 def ptr(t):

@@ -1,0 +1,280 @@
+// AdamW over many tensors with both moments in fp32, and the global 2-norm of many gradient tensors that clips it, beside the
+// FP8-state steps of adamw.hip.
+//
+//   n = sqrt(sum over all tensors of g^2);   s = min(1, max_norm / (n + 1e-6))
+//   g' = s g;   m = beta1 m + (1 - beta1) g';   v = beta2 v + (1 - beta2) g'^2
+//   p = p - lr (m / ((sqrt(v) / c2 + eps) c1) + wd p),   c1 = 1 - beta1^step,  c2 = sqrt(1 - beta2^step)
+// the order of operations of the FP8-state steps.  p is the fp32 master copy where there is one; the parameter of 16 bits is
+// then its rounding.  Everything is fp32; the sum of squares is taken in 64 bits (squares of fp32 gradients neither overflow
+// nor lose small tensors next to large ones, and the order of the additions no longer shows), in a fixed order: no atomics.
+//
+// Both kernels stream.  The records of the tensors travel in the kernel arguments (4 KB): no copy to the device ahead of the
+// launch, nothing that a captured graph would have to keep alive.
+#include <math.h>
+
+#include "coat_host.h"
+#include "elem_io.h"
+
+namespace coat {
+
+// ------------------------------------------------------------------------------------------------ sum of squares
+constexpr int kNormMax = 128;        // tensors per launch
+constexpr int kNormChunk = 8192;     // elements a block takes at a time
+constexpr int kNormBlocks = 2048;    // blocks (partial sums) per launch at most
+struct NormArgs {
+    const void* g[kNormMax];
+    int64_t numel[kNormMax];
+    uint32_t first_chunk[kNormMax + 1];  // first_chunk[count] = number of chunks
+    uint8_t dt[kNormMax];
+    int count;
+};
+
+// Index of the last tensor whose first chunk is not after `chunk` (wave-uniform).
+__device__ __forceinline__ int find_tensor(const uint32_t* first, int count, uint32_t chunk) {
+    int lo = 0, hi = count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (chunk >= first[mid]) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <int DT> __device__ __forceinline__ double sumsq_chunk(const void* g, int64_t begin, int64_t numel) {
+    double s = 0.0;
+#pragma unroll
+    for (int j = 0; j < kNormChunk / 2048; j++) {
+        const int64_t e = begin + j * 2048 + threadIdx.x * 8;
+        float v[8];
+        load8<DT>(elem_at<DT>(g, e), numel - e, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) s = fma((double)v[i], (double)v[i], s);
+    }
+    return s;
+}
+
+__device__ __forceinline__ double block_sum_f64(double s, double* red) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = red[0];
+    for (int k = 1; k < (int)(blockDim.x >> 6); k++) s += red[k];
+    return s;
+}
+
+__global__ __launch_bounds__(256) void k_grad_sumsq(NormArgs A, double* __restrict__ partial) {
+    __shared__ double red[4];
+    double s = 0.0;
+    const uint32_t chunks = A.first_chunk[A.count];
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int t = find_tensor(A.first_chunk, A.count, c);
+        const int64_t begin = (int64_t)(c - A.first_chunk[t]) * kNormChunk;
+        if (A.dt[t] == kF32) s += sumsq_chunk<kF32>(A.g[t], begin, A.numel[t]);
+        else if (A.dt[t] == kBF16) s += sumsq_chunk<kBF16>(A.g[t], begin, A.numel[t]);
+        else s += sumsq_chunk<kF16>(A.g[t], begin, A.numel[t]);
+    }
+    s = block_sum_f64(s, red);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+// out[0] = the norm, out[1] = the factor of the gradients.  A norm that is not a number gives a factor that is not one.
+__global__ __launch_bounds__(1024) void k_grad_norm(const double* __restrict__ partial, int64_t n, float max_norm, float* __restrict__ out) {
+    __shared__ double red[16];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += partial[i];
+    s = block_sum_f64(s, red);
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(s), f = (double)max_norm / (norm + 1e-6);
+        out[0] = (float)norm;
+        out[1] = f > 1.0 ? 1.0f : (float)f;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ the step
+constexpr int kStepMax = 64;        // tensors per launch
+constexpr int kStepChunk = 4096;    // elements a block steps
+struct Step32Tensor {
+    void* p;
+    const void* g;
+    float *m, *v, *master;
+    int64_t numel;
+};
+struct Step32Args {
+    Step32Tensor t[kStepMax];
+    uint32_t first_chunk[kStepMax + 1];
+    int count;
+    const float* grad_scale;
+};
+struct Hyper32 {
+    float beta1, one_minus_beta1, beta2, one_minus_beta2, lr, wd, eps, c1, inv_c2;
+};
+
+template <int PDT, int GDT, bool MASTER>
+__global__ __launch_bounds__(256) void k_adamw32(Step32Args A, Hyper32 H) {
+    const int ti = find_tensor(A.first_chunk, A.count, blockIdx.x);
+    const Step32Tensor T = A.t[ti];
+    const float gs = A.grad_scale ? *A.grad_scale : 1.0f;
+    const int64_t begin = (int64_t)(blockIdx.x - A.first_chunk[ti]) * kStepChunk;
+#pragma unroll
+    for (int j = 0; j < kStepChunk / 2048; j++) {
+        const int64_t e = begin + j * 2048 + threadIdx.x * 8, left = T.numel - e;
+        if (left <= 0) return;
+        float p[8], g[8], m[8], v[8];
+        if (MASTER) load8<kF32>(T.master + e, left, p);
+        else load8<PDT>(elem_at<PDT>(T.p, e), left, p);
+        load8<GDT>(elem_at<GDT>(T.g, e), left, g);
+        load8<kF32>(T.m + e, left, m);
+        load8<kF32>(T.v + e, left, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float gr = g[i] * gs;
+            m[i] = fmaf(H.beta1, m[i], H.one_minus_beta1 * gr);
+            v[i] = fmaf(H.beta2, v[i], (H.one_minus_beta2 * gr) * gr);
+            const float denom = fmaf(sqrtf(v[i]), H.inv_c2, H.eps) * H.c1;
+            const float update = fmaf(H.wd, p[i], m[i] / denom);
+            p[i] = fmaf(-H.lr, update, p[i]);
+        }
+        store8<kF32>(T.m + e, left, m);
+        store8<kF32>(T.v + e, left, v);
+        if (MASTER) store8<kF32>(T.master + e, left, p);
+        store8<PDT>(elem_at<PDT>(T.p, e), left, p);
+    }
+}
+
+}  // namespace coat
+
+using namespace coat;
+
+static bool opt_dtype(int dt) { return dt == COAT_F32 || dt == COAT_BF16 || dt == COAT_F16; }
+static bool elem_aligned(const void* p, int dt) { return ((uintptr_t)p & (dt == COAT_F32 ? 3u : 1u)) == 0; }
+static int64_t norm_chunks(int64_t numel) { return (numel + kNormChunk - 1) / kNormChunk; }
+
+// Calls fn(first, last, chunks) for each run of tensors that one launch takes: at most `most` tensors that are not empty and
+// fewer than 2^31 chunks.  Returns COAT_ESHAPE if one tensor alone has more.
+template <typename F> static int for_each_launch(int count, const int64_t* numel, int64_t chunk, int most, F fn) {
+    for (int i = 0; i < count;) {
+        const int first = i;
+        int used = 0;
+        int64_t chunks = 0;
+        for (; i < count && used < most; i++) {
+            if (numel[i] == 0) continue;
+            const int64_t c = (numel[i] + chunk - 1) / chunk;
+            if (chunks + c > 0x7fffffffll) {
+                if (used == 0) return COAT_ESHAPE;
+                break;
+            }
+            chunks += c;
+            used++;
+        }
+        if (used == 0) break;  // only empty tensors were left
+        if (const int rc = fn(first, i, chunks)) return rc;
+    }
+    return COAT_OK;
+}
+
+extern "C" int coat_grad_norm_partials(int count, const int64_t* numel) {
+    if (count < 0 || (count > 0 && !numel)) return COAT_EINVAL;
+    int64_t total = 0;
+    for (int i = 0; i < count; i++)
+        if (numel[i] < 0) return COAT_EINVAL;
+    const int rc = for_each_launch(count, numel, kNormChunk, kNormMax, [&](int, int, int64_t chunks) {
+        total += chunks < kNormBlocks ? chunks : kNormBlocks;
+        return total > 0x7fffffff ? COAT_ESHAPE : COAT_OK;
+    });
+    return rc != COAT_OK ? rc : (int)total;
+}
+
+extern "C" int coat_grad_norm_multi(int count, const void* const* grads, const int* dtypes, const int64_t* numel, float max_norm,
+                                    double* partial, int n_partial, float* out, void* stream) {
+    const int need = coat_grad_norm_partials(count, numel);
+    if (need < 0) return need;
+    if ((count > 0 && (!grads || !dtypes)) || !out || !(max_norm >= 0.0f)) return COAT_EINVAL;
+    if (need > 0 && (!partial || n_partial < need)) return COAT_EINVAL;
+    if (((uintptr_t)partial & 7u) || !elem_aligned(out, COAT_F32)) return COAT_EALIGN;
+    for (int i = 0; i < count; i++) {
+        if (!opt_dtype(dtypes[i])) return COAT_EDTYPE;
+        if (numel[i] == 0) continue;
+        if (!grads[i]) return COAT_EINVAL;
+        if (!elem_aligned(grads[i], dtypes[i])) return COAT_EALIGN;
+    }
+    hipStream_t st = (hipStream_t)stream;
+    double* at = partial;
+    const int rc = for_each_launch(count, numel, kNormChunk, kNormMax, [&](int first, int last, int64_t chunks) {
+        NormArgs A;
+        A.count = 0;
+        uint32_t c = 0;
+        for (int i = first; i < last; i++) {
+            if (numel[i] == 0) continue;
+            A.g[A.count] = grads[i];
+            A.numel[A.count] = numel[i];
+            A.dt[A.count] = (uint8_t)dtypes[i];
+            A.first_chunk[A.count++] = c;
+            c += (uint32_t)norm_chunks(numel[i]);
+        }
+        A.first_chunk[A.count] = c;
+        const int blocks = (int)(chunks < kNormBlocks ? chunks : kNormBlocks);
+        hipLaunchKernelGGL(k_grad_sumsq, dim3(blocks), dim3(256), 0, st, A, at);
+        at += blocks;
+        return coat_launch_status();
+    });
+    if (rc != COAT_OK) return rc;
+    hipLaunchKernelGGL(k_grad_norm, dim3(1), dim3(1024), 0, st, partial, (int64_t)need, max_norm, out);
+    return coat_launch_status();
+}
+
+extern "C" int coat_adamw_step_multi(int count, void* const* params, int p_dtype, const void* const* grads, int g_dtype,
+                                     float* const* exp_avg, float* const* exp_avg_sq, float* const* masters, const int64_t* numel,
+                                     const double* hyper, int step, const float* grad_scale, void* stream) {
+    if (count < 0) return COAT_EINVAL;
+    if (count == 0) return COAT_OK;
+    if (!params || !grads || !exp_avg || !exp_avg_sq || !numel || !hyper || step < 1) return COAT_EINVAL;
+    if (!opt_dtype(p_dtype) || (g_dtype != p_dtype && g_dtype != COAT_F32) || (masters && p_dtype == COAT_F32)) return COAT_EDTYPE;
+    if (!elem_aligned(grad_scale, COAT_F32)) return COAT_EALIGN;
+    for (int i = 0; i < count; i++) {  // everything is checked before the first launch
+        if (numel[i] < 0) return COAT_EINVAL;
+        if (numel[i] == 0) continue;
+        if (!params[i] || !grads[i] || !exp_avg[i] || !exp_avg_sq[i] || (masters && !masters[i])) return COAT_EINVAL;
+        if (!elem_aligned(params[i], p_dtype) || !elem_aligned(grads[i], g_dtype) || !elem_aligned(exp_avg[i], COAT_F32) ||
+            !elem_aligned(exp_avg_sq[i], COAT_F32) || (masters && !elem_aligned(masters[i], COAT_F32)))
+            return COAT_EALIGN;
+    }
+    // hyperparameters in double, rounded once: 1 - beta2 of a beta2 that was already rounded to fp32 is off by 1e-5 at 0.999
+    const double beta1 = hyper[0], beta2 = hyper[1];
+    Hyper32 H;
+    H.beta1 = (float)beta1;
+    H.one_minus_beta1 = (float)(1.0 - beta1);
+    H.beta2 = (float)beta2;
+    H.one_minus_beta2 = (float)(1.0 - beta2);
+    H.lr = (float)hyper[2];
+    H.wd = (float)hyper[3];
+    H.eps = (float)hyper[4];
+    H.c1 = (float)(1.0 - pow(beta1, (double)step));
+    H.inv_c2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+    hipStream_t st = (hipStream_t)stream;
+    return for_each_launch(count, numel, kStepChunk, kStepMax, [&](int first, int last, int64_t chunks) {
+        Step32Args A;
+        A.count = 0;
+        A.grad_scale = grad_scale;
+        uint32_t c = 0;
+        for (int i = first; i < last; i++) {
+            if (numel[i] == 0) continue;
+            A.t[A.count] = Step32Tensor{params[i], grads[i], exp_avg[i], exp_avg_sq[i], masters ? masters[i] : nullptr, numel[i]};
+            A.first_chunk[A.count++] = c;
+            c += (uint32_t)((numel[i] + kStepChunk - 1) / kStepChunk);
+        }
+        A.first_chunk[A.count] = c;
+        const dim3 grid((unsigned)chunks), block(256);
+#define STEP(PDT, GDT, MASTER) hipLaunchKernelGGL((k_adamw32<PDT, GDT, MASTER>), grid, block, 0, st, A, H)
+        if (p_dtype == COAT_F32) STEP(kF32, kF32, false);
+        else if (p_dtype == COAT_BF16) {
+            if (masters) { if (g_dtype == COAT_F32) STEP(kBF16, kF32, true); else STEP(kBF16, kBF16, true); }
+            else { if (g_dtype == COAT_F32) STEP(kBF16, kF32, false); else STEP(kBF16, kBF16, false); }
+        } else {
+            if (masters) { if (g_dtype == COAT_F32) STEP(kF16, kF32, true); else STEP(kF16, kF16, true); }
+            else { if (g_dtype == COAT_F32) STEP(kF16, kF32, false); else STEP(kF16, kF16, false); }
+        }
+#undef STEP
+        return coat_launch_status();
+    });
+}

@@ -1,0 +1,85 @@
+// Wide loads and stores of 16- and 32-bit elements at any element alignment, for the kernels that take row slices, odd row
+// lengths and tensors laid out one after the other without padding.  The hardware's global loads and stores need no more
+// than the element's own alignment (the code objects run in unaligned access mode), so a 16-byte access that crosses a line
+// costs one more line, not a loop over elements: only the last, incomplete piece of a row goes element by element.
+#pragma once
+#include "coat_device.h"
+
+namespace coat {
+
+typedef uint32_t coat_u4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t coat_u2_at2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t coat_u4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+
+template <int DT> struct ElemBytes { static constexpr int value = DT == kF32 ? 4 : 2; };
+template <int DT> __device__ __forceinline__ const void* elem_at(const void* p, int64_t i) { return (const char*)p + i * ElemBytes<DT>::value; }
+template <int DT> __device__ __forceinline__ void* elem_at(void* p, int64_t i) { return (char*)p + i * ElemBytes<DT>::value; }
+
+template <int DT> __device__ __forceinline__ float elem_lo(uint32_t w) { return DT == kBF16 ? bf16lo(w) : f16lo(w); }
+template <int DT> __device__ __forceinline__ float elem_hi(uint32_t w) { return DT == kBF16 ? bf16hi(w) : f16hi(w); }
+template <int DT> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    return DT == kBF16 ? pack_bf16x2(lo, hi) : (f2f16(lo) | (f2f16(hi) << 16));
+}
+
+// Eight elements as they lie in memory (16 bytes of 16-bit elements, 32 of fp32), kept packed until they are used.
+template <int DT> struct Raw8 { uint32_t w[DT == kF32 ? 8 : 4]; };
+
+// p: address of the first element; left: elements from there to the end of the row (<= 0: nothing is read, zeros).
+template <int DT> __device__ __forceinline__ Raw8<DT> load_raw8(const void* p, int64_t left) {
+    Raw8<DT> r;
+    if (left >= 8) {
+        if (DT == kF32) {
+            const coat_u4_at4 a = ((const coat_u4_at4*)p)[0], b = ((const coat_u4_at4*)p)[1];
+            r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
+            r.w[DT == kF32 ? 4 : 0] = b.x; r.w[DT == kF32 ? 5 : 1] = b.y; r.w[DT == kF32 ? 6 : 2] = b.z; r.w[DT == kF32 ? 7 : 3] = b.w;
+        } else {
+            const coat_u4_at2 a = *(const coat_u4_at2*)p;
+            r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < left) {
+                if (DT == kF32) r.w[DT == kF32 ? i : 0] = ((const uint32_t*)p)[i];
+                else r.w[i >> 1] |= (uint32_t)((const uint16_t*)p)[i] << (16 * (i & 1));
+            }
+    }
+    return r;
+}
+template <int DT> __device__ __forceinline__ void raw8_to_f32(const Raw8<DT>& r, float* o) {
+    if (DT == kF32) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = u2f(r.w[DT == kF32 ? i : 0]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            o[2 * k] = elem_lo<DT>(r.w[k]);
+            o[2 * k + 1] = elem_hi<DT>(r.w[k]);
+        }
+    }
+}
+template <int DT> __device__ __forceinline__ void load8(const void* p, int64_t left, float* o) { raw8_to_f32<DT>(load_raw8<DT>(p, left), o); }
+template <int DT> __device__ __forceinline__ void store8(void* p, int64_t left, const float* v) {
+    if (left >= 8) {
+        if (DT == kF32) {
+            ((coat_u4_at4*)p)[0] = (coat_u4_at4){f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])};
+            ((coat_u4_at4*)p)[1] = (coat_u4_at4){f2u(v[4]), f2u(v[5]), f2u(v[6]), f2u(v[7])};
+        } else {
+            *(coat_u4_at2*)p = (coat_u4_at2){pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7])};
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < left) store_from_f32<DT>(p, i, v[i]);
+    }
+}
+// The same with the element type known at run time only (weights and biases): a wave-uniform branch.
+__device__ __forceinline__ void load8_rt(const void* p, int dt, int64_t i, int64_t n, float* o) {
+    if (dt == kF32) load8<kF32>(elem_at<kF32>(p, i), n - i, o);
+    else if (dt == kBF16) load8<kBF16>(elem_at<kBF16>(p, i), n - i, o);
+    else load8<kF16>(elem_at<kF16>(p, i), n - i, o);
+}
+
+}  // namespace coat

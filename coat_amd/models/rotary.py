@@ -1,0 +1,130 @@
+"""Rotary positions with several axes (time, height, width of video, image and text tokens) on q and k together, beside the one-axis
+rotary of the decoder layers (``coat_llama.fused_rotary``).  Kernel: coat_amd/csrc/rope_axes.hip."""
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _hip
+
+
+class RotaryAxes:
+    """Which pair of a head turns with which axis, and how fast.
+
+    ``sections``: pairs of each axis in turn; their sum P is the number of turning pairs, 2 P <= ``head_dim`` (the elements behind
+    are passed through).  Pair j turns by ``position * theta ** -(j / P)``; with ``restart`` every section counts its own pairs,
+    ``theta ** -(i / n)`` for pair i of a section of n.  Pair j is elements ``(j, j + P)`` of the head, the layout of the decoder
+    layers; with ``pairs`` neighbours ``(2 j, 2 j + 1)``.  The tables live on the device that is current at construction; another
+    device gets its own at the first use there (which must not be inside a graph capture)."""
+
+    def __init__(self, head_dim, sections, theta=10000.0, restart=False, pairs=False):
+        self.head_dim, self.sections, self.theta = int(head_dim), tuple(int(n) for n in sections), float(theta)
+        self.restart, self.pairs = bool(restart), bool(pairs)
+        if not self.sections or min(self.sections) < 0 or sum(self.sections) < 1:
+            raise ValueError(f"RotaryAxes: invalid sections {tuple(sections)}")
+        if 2 * sum(self.sections) > self.head_dim:
+            raise ValueError(f"RotaryAxes: sections {self.sections} hold more pairs than a head of {self.head_dim}")
+        if not (self.theta > 0.0 and math.isfinite(self.theta)):
+            raise ValueError(f"RotaryAxes: invalid theta {theta}")
+        total = sum(self.sections)
+        self._axis = [a for a, n in enumerate(self.sections) for _ in range(n)]
+        exponent = [i / n for n in self.sections for i in range(n)] if self.restart else [j / total for j in range(total)]
+        self._freq = [self.theta ** -e for e in exponent]  # radians a position, in 64 bits
+        self._tables = {}
+        if torch.cuda.is_available():
+            self.tables(torch.device("cuda", torch.cuda.current_device()))
+
+    def tables(self, device):
+        """(turns a position fp64 [P], axis int32 [P]) on ``device``."""
+        if device not in self._tables:
+            turns = torch.tensor([f / (2.0 * math.pi) for f in self._freq], dtype=torch.float64, device=device)
+            self._tables[device] = turns, torch.tensor(self._axis, dtype=torch.int32, device=device)
+        return self._tables[device]
+
+    def cos_sin(self, position_ids, dtype):
+        """cos / sin [B, S, 2 P] for the (j, j + P) layout, from torch operations on any device; position_ids [axes, B, S]."""
+        freq = torch.tensor(self._freq, dtype=torch.float64, device=position_ids.device)
+        angle = position_ids[torch.tensor(self._axis, device=position_ids.device)].permute(1, 2, 0).double() * freq
+        angle = torch.cat((angle, angle), -1)
+        return angle.cos().to(dtype), angle.sin().to(dtype)
+
+
+def _positions(position_ids, plan, B, S, device):
+    if position_ids.dim() != 3 or position_ids.shape[0] != len(plan.sections):
+        raise ValueError(f"rotary_axes: expected position_ids of shape [{len(plan.sections)}, batch, seq], got {tuple(position_ids.shape)}")
+    if position_ids.device != device:
+        raise ValueError(f"rotary_axes: position_ids are on {position_ids.device}, q and k on {device}")
+    if position_ids.dtype != torch.int64:
+        if position_ids.dtype.is_floating_point or position_ids.dtype.is_complex or position_ids.dtype == torch.bool:
+            raise ValueError(f"rotary_axes: position_ids must be whole numbers, got {position_ids.dtype}")
+        position_ids = position_ids.long()
+    return position_ids.expand(-1, B, S)
+
+
+def _rotate(q, k, position_ids, plan, inverse):
+    given = [t for t in (q, k) if t is not None]
+    if not given:
+        raise ValueError("rotary_axes: neither q nor k given")
+    first = given[0]
+    if not first.is_cuda:
+        raise RuntimeError("coat_amd kernels need tensors on the GPU (got a %s tensor)" % first.device.type)
+    for t in given:
+        if t.dim() != 4 or t.shape[:2] != first.shape[:2] or t.shape[3] != plan.head_dim:
+            raise ValueError(f"rotary_axes: expected [batch, seq, heads, {plan.head_dim}] tensors of one batch, got {tuple(t.shape)}")
+        if t.dtype != first.dtype or t.device != first.device:
+            raise ValueError("rotary_axes: q and k must have one dtype and device")
+    B, S, _, D = first.shape
+    device = first.device
+    pos = _positions(position_ids, plan, B, S, device)
+    turns, axis = plan.tables(device)
+    args, outs, kept = [], [], []
+    for t in (q, k):
+        if t is None:
+            args += [None, None, 0, 0, 0, 0]
+            outs.append(None)
+            continue
+        if t.stride(3) != 1 and D > 1:
+            t = t.contiguous()
+        kept.append(t)
+        out = torch.empty(t.shape, dtype=t.dtype, device=device)
+        args += [t.data_ptr(), out.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2]]
+        outs.append(out)
+    _hip.launch("coat_rope_axes", device, *args, _hip.dt(first), pos.data_ptr(), *pos.stride(), len(plan.sections), turns.data_ptr(),
+                axis.data_ptr(), sum(plan.sections), D, 1 if plan.pairs else 0, 1 if inverse else 0, B, S, what="rotary_axes")
+    return outs[0], outs[1]
+
+
+def rotary_axes_forward(q, k, position_ids, plan):
+    """Rotates q [B, S, heads, head_dim] and k [B, S, kv_heads, head_dim] (either may be None; bf16, fp16 or fp32; any strides, such
+    as slices of a fused projection) by position_ids [axes, B, S] (whole numbers, broadcast over B and S).  Returns new dense
+    tensors of the same shapes.  Angles are taken in 64 bits, the rotation in fp32, rounded once."""
+    return _rotate(q, k, position_ids, plan, False)
+
+
+def rotary_axes_backward(dq, dk, position_ids, plan):
+    """The gradients of ``rotary_axes_forward``'s q and k: the rotation by the negated angles."""
+    return _rotate(dq, dk, position_ids, plan, True)
+
+
+class _RotaryAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, position_ids, plan):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(position_ids)
+        ctx.plan = plan
+        return _rotate(q, k, position_ids, plan, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk):
+        if dq is None and dk is None:
+            return None, None, None, None
+        (position_ids,) = ctx.saved_tensors
+        return (*_rotate(dq, dk, position_ids, ctx.plan, True), None, None)
+
+
+def rotary_axes(q, k, position_ids, plan):
+    """``rotary_axes_forward`` with autograd."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+        return _RotaryAxes.apply(q, k, position_ids, plan)
+    return rotary_axes_forward(q, k, position_ids, plan)

@@ -116,3 +116,88 @@ def fp8_adamw_step_multi(params, grads, exp_avg, scale_exp_avg, exp_avg_sq, scal
     """``fp8_adamw_step`` on lists of tensors: one launch per 32 tensors."""
     _multi(False, params, grads, exp_avg, exp_avg_sq, (scale_exp_avg, scale_exp_avg_sq), (beta1, beta2, lr, wd, eps), step,
            qgroup_size, 0)
+
+
+# ------------------------------------------------------------------------------------------------ 32-bit states, clipping
+def _columns(what, lists):
+    """Checks parallel lists of tensors (name, tensors, dtypes allowed or None) that a multi-tensor call reads or writes flat: one
+    length, one device, one dtype a list, equal sizes, contiguous.  Returns (device, sizes, addresses of each list)."""
+    first = lists[0][1]
+    n, index = len(first), first[0].get_device()
+    if index < 0:
+        raise RuntimeError(f"{what}: tensors must be on the GPU")
+    numel, out = list(map(torch.Tensor.numel, first)), []
+    for name, tensors, dtype in lists:
+        if len(tensors) != n:
+            raise RuntimeError(f"{what}: the tensor lists differ in length")
+        if set(map(torch.Tensor.get_device, tensors)) != {index}:
+            raise RuntimeError(f"{what}: {name} holds tensors that are not on the first tensor's device")
+        if dtype is not None and {t.dtype for t in tensors} != {dtype}:
+            raise RuntimeError(f"{what}: {name} must all be {dtype}")
+        if list(map(torch.Tensor.numel, tensors)) != numel:
+            raise RuntimeError(f"{what}: sizes of {name} differ from those of {lists[0][0]}")
+        if not all(map(torch.Tensor.is_contiguous, tensors)):
+            raise RuntimeError(f"{what}: {name} must be contiguous")
+        out.append(list(map(torch.Tensor.data_ptr, tensors)))
+    return first[0].device, numel, out
+
+
+def grad_norm_multi(grads, max_norm=None):
+    """The 2-norm of all ``grads`` (fp32 / bf16 / fp16 GPU tensors) taken together, and the factor that clips them to ``max_norm``.
+
+    Returns ``(norm, scale)``: 0-dim fp32 tensors on the device, ``scale = min(1, max_norm / (norm + 1e-6))``, or None without
+    ``max_norm``.  The gradients are only read: pass ``scale`` as ``grad_scale`` to the step.  Squares are summed in 64 bits and a
+    fixed order.  A norm that is infinite gives the factor 0, one that is not a number a factor that is not one, as
+    ``torch.nn.utils.clip_grad_norm_`` does."""
+    grads = list(grads)
+    if max_norm is not None and not float(max_norm) >= 0.0:
+        raise ValueError(f"grad_norm_multi: invalid max_norm {max_norm}")
+    if not grads:
+        raise ValueError("grad_norm_multi: no gradients")
+    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    n = len(grads)
+    device, numel, (addresses,) = _columns("grad_norm_multi", [("grads", grads, None)])
+    dtypes = (ctypes.c_int * n)(*[_hip.dt(g) for g in grads])
+    numel = (ctypes.c_int64 * n)(*numel)
+    parts = _hip.lib().coat_grad_norm_partials(n, numel)
+    if parts < 0:
+        _hip.check(parts, "grad_norm_multi")
+    work = torch.empty(max(parts, 1), dtype=torch.float64, device=device)
+    out = torch.empty(2, dtype=torch.float32, device=device)
+    _hip.launch("coat_grad_norm_multi", device, n, (ctypes.c_void_p * n)(*addresses), dtypes, numel,
+                0.0 if max_norm is None else float(max_norm), work.data_ptr(), parts, out.data_ptr(), what="grad_norm_multi")
+    norm, scale = out.unbind()
+    return norm, None if max_norm is None else scale
+
+
+def adamw_step_multi(params, grads, exp_avg, exp_avg_sq, beta1, beta2, lr, wd, eps, step, masters=None, grad_scale=None):
+    """AdamW on lists of tensors with both moments in fp32, in place: one launch per 64 tensors, the formula of
+    ``fp8_adamw_step``.  ``params`` share a dtype, ``grads`` have theirs or fp32.  ``masters``: fp32 copies of 16-bit parameters;
+    they are stepped, and the parameters receive their rounding.  ``grad_scale``: a one-element fp32 tensor on the device that the
+    gradients are multiplied by (``grad_norm_multi``).  ``step`` counts from 1 and is read on the host: a captured graph keeps it."""
+    n = len(params)
+    if n == 0:
+        return
+    lists = [("params", params, params[0].dtype), ("grads", grads, grads[0].dtype if len(grads) else None),
+             ("exp_avg", exp_avg, torch.float32), ("exp_avg_sq", exp_avg_sq, torch.float32)]
+    if masters is not None:
+        lists.append(("masters", masters, torch.float32))
+    device, numel, addresses = _columns("adamw_step_multi", lists)
+    pdt, gdt = params[0].dtype, grads[0].dtype
+    if gdt != pdt and gdt != torch.float32:
+        raise RuntimeError(f"adamw_step_multi: grads dtype {gdt} is neither the params' {pdt} nor torch.float32")
+    if masters is not None and pdt == torch.float32:
+        raise RuntimeError("adamw_step_multi: masters are for parameters of 16 bits")
+    written = [a for column in addresses[:1] + addresses[2:] for a, size in zip(column, numel) if size]
+    if len(set(written)) != len(written):
+        raise RuntimeError("adamw_step_multi: a tensor that is stepped is given twice")
+    if not int(step) >= 1:
+        raise ValueError(f"adamw_step_multi: invalid step {step}")
+    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != device):
+        raise RuntimeError("adamw_step_multi: grad_scale must be one fp32 element on the parameters' device")
+    arrays = [(ctypes.c_void_p * n)(*a) for a in addresses]
+    _hip.launch("coat_adamw_step_multi", device, n, arrays[0], _hip.dt(pdt), arrays[1], _hip.dt(gdt), arrays[2], arrays[3],
+                arrays[4] if masters is not None else None, (ctypes.c_int64 * n)(*numel), (ctypes.c_double * 5)(beta1, beta2, lr, wd, eps),
+                int(step), None if grad_scale is None else grad_scale.data_ptr(), what="adamw_step_multi")
+    # written behind autograd's back: graphs that saved them must notice
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])

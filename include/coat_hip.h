@@ -48,9 +48,10 @@ enum coat_fp8 { COAT_E4M3 = 0, COAT_E5M2 = 1 }; /* torch.float8_e4m3fn / torch.f
 /* Bumped whenever an entry point's argument list or the size of a buffer it writes changes (2: every s_max / amax
  * argument became COAT_MAX_WORDS words; 3: coat_fp8_gemm_residual, coat_fp8_rmsnorm_backward_add and coat_attention_forward_bf16 added,
  * coat_hbm_probe removed; 4: coat_rope_bf16 and coat_attention_forward_bf16 take a maximum buffer, the multi-tensor optimizer
- * steps and coat_fp8_layernorm_backward_add added; 5: coat_fp8_quantize_perblock added).  A caller compiled against this header checks coat_abi_version() == COAT_ABI_VERSION when it
+ * steps and coat_fp8_layernorm_backward_add added; 5: coat_fp8_quantize_perblock added;
+ * 6: coat_layer_norm_*, coat_rope_axes, coat_grad_norm_* and coat_adamw_step_multi added).  A caller compiled against this header checks coat_abi_version() == COAT_ABI_VERSION when it
  * loads the library. */
-#define COAT_ABI_VERSION 5
+#define COAT_ABI_VERSION 6
 int coat_abi_version(void);
 const char* coat_version(void);
 const char* coat_status_string(int status);
@@ -286,6 +287,36 @@ int coat_rope_bf16(const void* x, void* y, const float* cos_tab, const float* si
                    const int64_t* pos, int64_t rows, int seq_len, int heads, int head_dim, int inverse, int64_t x_pitch,
                    int64_t y_pitch, float* s_max, int fp8_max, void* stream);
 
+/* Rotary positions with several axes (time, height, width, ...), q and k in one launch; no counterpart in the reference.
+ * q / k [batch, seq, heads, head_dim] of `dtype`, addressed through element strides (batch, token, head; the head dimension is
+ * contiguous); q_out / k_out dense, never the inputs' memory.  Either may have 0 heads (pointers then ignored).
+ * pos int64 [axes, batch, seq] with element strides (a stride may be 0), any values.  Pair j of `pairs` (2 * pairs <= head_dim)
+ * turns by pos[axis[j]] * turns[j] whole turns: turns fp64 [pairs] = frequency / (2 pi), axis int32 [pairs] in [0, axes), both in
+ * device memory.  adjacent 0: pair j is elements (j, j + pairs); 1: (2j, 2j + 1).  Elements from 2 * pairs on are copied.
+ * inverse 1: the negated angle, which is the backward pass.  Angles are reduced in fp64, the rotation is fp32, rounded once.
+ * Addresses need the element's own alignment only.  head_dim <= 2048, at most 4096 heads each. */
+int coat_rope_axes(const void* q, void* q_out, int64_t q_sb, int64_t q_ss, int64_t q_sh, int q_heads, const void* k, void* k_out,
+                   int64_t k_sb, int64_t k_ss, int64_t k_sh, int k_heads, int dtype, const int64_t* pos, int64_t pos_sa,
+                   int64_t pos_sb, int64_t pos_ss, int axes, const double* turns, const int32_t* axis, int pairs, int head_dim,
+                   int adjacent, int inverse, int64_t batch, int64_t seq, void* stream);
+
+/* ---- LayerNorm of 16- and 32-bit tensors ----------------------------------------------------------------
+ * The norms outside the FP8 blocks (no counterpart in the reference, which leaves them to torch).
+ * y = (x - mean) * rstd (* w (+ b)) over the last dimension; x [M, N] of x_dtype with a row pitch in elements (0 = N), y dense;
+ * w, b [N] of w_dtype, w NULL: no affine parameters, b NULL: no bias; mean, rstd fp32 [M].  Any N >= 1; addresses need the
+ * element's own alignment only.  Sums are fp32, the variance is the two-pass one, y is rounded once. */
+int coat_layer_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const void* w, const void* b, int w_dtype, void* y,
+                            float* mean, float* rstd, int64_t M, int64_t N, float eps, void* stream);
+/* Partial rows that coat_layer_norm_backward makes use of for such a tensor (the n_partial to allocate), or a negative status. */
+int coat_layer_norm_partials(int64_t M, int64_t N);
+/* dx (dense, x_dtype), dw and db (w_dtype), each optional (NULL).  dy, x of x_dtype with row pitches (0 = N).  partial: fp32
+ * workspace [2, n_partial, N] if both dw and db are wanted, [1, n_partial, N] for one, unused for none; 1 <= n_partial <= 65535,
+ * more than coat_layer_norm_partials(M, N) are not used.  The partial rows are summed in a fixed order: the same bits every time
+ * for one n_partial.  M = 0 gives zero gradients. */
+int coat_layer_norm_backward(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, int x_dtype, const float* mean,
+                             const float* rstd, const void* w, int w_dtype, void* dx, void* dw, void* db, float* partial,
+                             int n_partial, int64_t M, int64_t N, void* stream);
+
 /* ---- bf16 attention (forward) ------------------------------------------------------------------------
  * The attention between the FP8 projections: the reference calls the flash-attn library here
  * (coat/models/coat_llama.py:960-971, used by LlamaAttentionWithoutLinear :981-1074).
@@ -373,6 +404,25 @@ int coat_fp8_adamw_step_multi(int count, void* const* params, const void* const*
                               float* const* scale_exp_avg, void* const* exp_avg_sq, float* const* scale_exp_avg_sq,
                               const int64_t* numel, const int64_t* n_scale, float beta1, float beta2, float lr, float wd,
                               float eps, int step, int qgroup_size, void* stream);
+
+/* The 2-norm of `count` gradient tensors taken together, and the factor that clips them to max_norm; no counterpart in the
+ * reference.  grads, dtypes, numel: host arrays, read before the call returns (a tensor may be empty).  out: two fp32 in device
+ * memory, out[0] = sqrt(sum of squares), out[1] = min(1, max_norm / (out[0] + 1e-6)) (not a number if the norm is not one).
+ * The sum is fp64 in a fixed order.  partial: fp64 workspace of coat_grad_norm_partials(count, numel) elements (which returns a
+ * negative status for bad sizes). */
+int coat_grad_norm_partials(int count, const int64_t* numel);
+int coat_grad_norm_multi(int count, const void* const* grads, const int* dtypes, const int64_t* numel, float max_norm,
+                         double* partial, int n_partial, float* out, void* stream);
+
+/* AdamW step of several tensors with both moments in fp32, 64 tensors to a launch; the formula of coat_fp8_adamw_step_multi.
+ * params of p_dtype; grads of p_dtype or fp32; masters NULL, or fp32 copies of 16-bit parameters that are stepped instead, the
+ * parameter receiving their rounding.  hyper: host array of five doubles: beta1, beta2, lr, weight decay, eps.  grad_scale: NULL,
+ * or one fp32 in device memory that the gradients are multiplied by (out[1] above).  Host arrays are read before the call
+ * returns; addresses need the element's own alignment only; the tensors that are written must not overlap; empty ones are
+ * skipped; everything is checked before the first launch. */
+int coat_adamw_step_multi(int count, void* const* params, int p_dtype, const void* const* grads, int g_dtype, float* const* exp_avg,
+                          float* const* exp_avg_sq, float* const* masters, const int64_t* numel, const double* hyper, int step,
+                          const float* grad_scale, void* stream);
 
 /* coat/activation/liger/cross_entropy.py:24-198 liger_cross_entropy_kernel as launched by cross_entropy_forward
  * (:212-278): softmax cross-entropy over x [n_rows, n_cols] (row pitch x_stride elements, fp32 / bf16 / fp16).
