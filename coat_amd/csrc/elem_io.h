@@ -8,7 +8,6 @@
 namespace coat {
 
 typedef uint32_t coat_u4_at2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t coat_u2_at2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t coat_u4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int DT> struct ElemBytes { static constexpr int value = DT == kF32 ? 4 : 2; };
@@ -36,17 +35,55 @@ template <int DT> __device__ __forceinline__ Raw8<DT> load_raw8(const void* p, i
             const coat_u4_at2 a = *(const coat_u4_at2*)p;
             r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
         }
+    } else if (left > 0) {  // all loads in flight together: elements past the end are read from the last one and cleared
+        uint32_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int64_t at = i < left ? i : left - 1;
+            e[i] = DT == kF32 ? ((const uint32_t*)p)[at] : ((const uint16_t*)p)[at];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) e[i] = i < left ? e[i] : 0u;
+#pragma unroll
+        for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = DT == kF32 ? e[k] : e[2 * k & 7] | e[(2 * k + 1) & 7] << 16;
     } else {
 #pragma unroll
         for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < left) {
-                if (DT == kF32) r.w[DT == kF32 ? i : 0] = ((const uint32_t*)p)[i];
-                else r.w[i >> 1] |= (uint32_t)((const uint16_t*)p)[i] << (16 * (i & 1));
-            }
     }
     return r;
+}
+// The same for a load that is issued well before its use: the last piece of a row is read as the eight elements that end the row,
+// and settle_row8 moves them to their places when they are used.  (Picking single elements needs their values, that is a wait
+// right after the load: one lane of a block then holds up every row, 1.8x the time at 4100 columns.)
+template <int DT> __device__ __forceinline__ Raw8<DT> load_row8(const void* row, int c, int n, bool valid) {
+    Raw8<DT> r;
+#pragma unroll
+    for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = 0;
+    if (valid && c < n) {
+        if (n >= 8) {
+            r = load_raw8<DT>(elem_at<DT>(row, c + 8 <= n ? c : n - 8), 8);
+        } else {
+            r = load_raw8<DT>(elem_at<DT>(row, c), n - c);
+        }
+    }
+    return r;
+}
+template <int DT> __device__ __forceinline__ void settle_row8(Raw8<DT>& r, int c, int n) {
+    const int past = c + 8 - n;  // elements of this piece past the end of the row
+    if (past > 0 && past < 8 && n >= 8) {
+        constexpr int W = DT == kF32 ? 8 : 4;
+        if (DT != kF32 && (past & 1)) {
+#pragma unroll
+            for (int k = 0; k < W; k++) r.w[k] = r.w[k] >> 16 | (k + 1 < W ? r.w[(k + 1) % W] << 16 : 0u);
+        }
+        const int words = past >> (DT == kF32 ? 0 : 1);
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1)
+            if (words & d) {
+#pragma unroll
+                for (int k = 0; k < W; k++) r.w[k] = k + d < W ? r.w[(k + d) % W] : 0u;
+            }
+    }
 }
 template <int DT> __device__ __forceinline__ void raw8_to_f32(const Raw8<DT>& r, float* o) {
     if (DT == kF32) {

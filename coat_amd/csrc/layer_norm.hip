@@ -9,6 +9,8 @@
 // kernel adds the partial rows in a fixed order: no atomics, the same bits on every run.
 #include <math.h>
 
+#include <type_traits>
+
 #include "coat_host.h"
 #include "elem_io.h"
 
@@ -25,6 +27,237 @@ template <int W> __device__ __forceinline__ float block_sum(float v, float* red)
 #pragma unroll
     for (int k = 1; k < W; k++) s += red[k];
     return s;
+}
+
+// ------------------------------------------------------------------------------------------------ rows held in registers
+// L lanes work on a row and hold C pieces of 8 elements each: piece k of lane l begins at column (k lanes + l) 8, so that the
+// lanes of a wave read one run of memory.  L = 8 .. 64: a wave works on 64 / L rows at a time and no barrier is needed.
+// L = kBlock: the block works on one row with as many waves as that takes.  The weights stay in registers over the rows of a
+// block, and the next row's loads are issued before the sums of the present one are exchanged.
+// RAGGED: N is not a multiple of 8; the last piece of a row is then incomplete.
+constexpr int kBlock = 0;
+constexpr int form_threads(int L, int C) { return L != kBlock ? 256 : C <= 2 ? 1024 : 512; }  // launch bound
+constexpr int form_rows(int L) { return L != kBlock ? 256 / L : 1; }                          // rows at a time
+
+// Sum over the lanes of a row, in each of them.  Block form: `red` holds 16 floats, zero beyond the block's waves; a buffer may be
+// used again after another buffer's exchange (whose barrier every wave reaches only after it has read this one).
+template <int L> __device__ __forceinline__ float row_sum(float v, float* red) {
+    if (L != kBlock) return cluster_sum<L ? L : 1>(v);
+    v = cluster_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return cluster_sum<16>(red[threadIdx.x & 15]);
+}
+template <int DT, bool RAGGED> __device__ __forceinline__ Raw8<DT> load_piece(const void* row, int c, int N, bool valid) {
+    if (RAGGED) return load_row8<DT>(row, c, N, valid);
+    Raw8<DT> r;
+#pragma unroll
+    for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = 0;
+    if (valid && c < N) r = load_raw8<DT>(elem_at<DT>(row, c), 8);
+    return r;
+}
+
+template <int DT, int L, int C, bool RAGGED>
+__global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __restrict__ x, int64_t x_pitch, const void* __restrict__ w,
+                                                                 const void* __restrict__ b, int w_dt, void* __restrict__ y,
+                                                                 float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t M,
+                                                                 int N, float eps) {
+    constexpr int R = form_rows(L);
+    __shared__ float red[2][16];
+    const int lanes = L == kBlock ? blockDim.x : L;
+    const int l = L == kBlock ? threadIdx.x : threadIdx.x % (L ? L : 1), r = L == kBlock ? 0 : threadIdx.x / (L ? L : 1);
+    const int64_t step = (int64_t)gridDim.x * R;
+    int64_t row = (int64_t)blockIdx.x * R + r;
+    const int64_t rounds = (M - (int64_t)blockIdx.x * R + step - 1) / step;  // the same for the whole block
+    const float inv_n = 1.0f / (float)N;
+    if (L == kBlock) {
+        if (threadIdx.x < 32) red[threadIdx.x >> 4][threadIdx.x & 15] = 0.0f;
+        __syncthreads();
+    }
+    Raw8<DT> raw[C];
+    float wv[C][8], bv[C][8];
+#pragma unroll
+    for (int k = 0; k < C; k++) raw[k] = load_piece<DT, RAGGED>(elem_at<DT>(x, row * x_pitch), (k * lanes + l) * 8, N, row < M);
+#pragma unroll
+    for (int k = 0; k < C; k++) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            wv[k][j] = 1.0f;
+            bv[k][j] = 0.0f;
+        }
+        if (w) load8_rt(w, w_dt, (k * lanes + l) * 8, N, wv[k]);
+        if (b) load8_rt(b, w_dt, (k * lanes + l) * 8, N, bv[k]);
+    }
+    for (int64_t i = 0; i < rounds; i++, row += step) {
+        float v[C][8], s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            if (RAGGED) settle_row8<DT>(raw[k], (k * lanes + l) * 8, N);
+            raw8_to_f32<DT>(raw[k], v[k]);
+            s += ((v[k][0] + v[k][1]) + (v[k][2] + v[k][3])) + ((v[k][4] + v[k][5]) + (v[k][6] + v[k][7]));
+        }
+        if (i + 1 < rounds) {
+            const int64_t next = row + step;
+#pragma unroll
+            for (int k = 0; k < C; k++)
+                raw[k] = load_piece<DT, RAGGED>(elem_at<DT>(x, next * x_pitch), (k * lanes + l) * 8, N, next < M);
+        }
+        const float mean = row_sum<L>(s, red[0]) * inv_n;
+        s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            const int left = N - (k * lanes + l) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                v[k][j] -= mean;
+                const float d = (RAGGED ? j : 0) < left ? v[k][j] : 0.0f;
+                s = fmaf(d, d, s);
+            }
+        }
+        const float rstd = 1.0f / sqrtf(row_sum<L>(s, red[1]) * inv_n + eps);
+        if (row < M) {
+#pragma unroll
+            for (int k = 0; k < C; k++) {
+                const int c = (k * lanes + l) * 8;
+                if (c >= N) continue;
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[k][j] = fmaf(v[k][j] * rstd, wv[k][j], bv[k][j]);
+                store8<DT>(elem_at<DT>(y, row * N + c), RAGGED ? N - c : 8, v[k]);
+            }
+            if (l == 0) {
+                mean_out[row] = mean;
+                rstd_out[row] = rstd;
+            }
+        }
+    }
+}
+
+// dx, and with SUMS one partial row of dw and db per block (pw / pb may be NULL).
+template <int DT, int L, int C, bool RAGGED, bool SUMS>
+__global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __restrict__ dy, int64_t dy_pitch, const void* __restrict__ x,
+                                                                 int64_t x_pitch, const float* __restrict__ mean_in,
+                                                                 const float* __restrict__ rstd_in, const void* __restrict__ w, int w_dt,
+                                                                 void* __restrict__ dx, float* __restrict__ pw, float* __restrict__ pb,
+                                                                 int64_t M, int N) {
+    constexpr int R = form_rows(L);
+    constexpr bool kShared = SUMS && R > 1;  // several rows of the block share a column: summed through LDS at the end
+    constexpr bool kLean = C * (DT == kF32 ? 2 : 1) * (RAGGED ? 2 : 1) >= 8;  // no registers left for the next row
+    __shared__ float red[4][16];
+    __shared__ float cols[kShared ? R : 1][kShared ? L * C * 8 : 1];
+    const int lanes = L == kBlock ? blockDim.x : L;
+    const int l = L == kBlock ? threadIdx.x : threadIdx.x % (L ? L : 1), r = L == kBlock ? 0 : threadIdx.x / (L ? L : 1);
+    const int64_t step = (int64_t)gridDim.x * R;
+    int64_t row = (int64_t)blockIdx.x * R + r;
+    const int64_t rounds = (M - (int64_t)blockIdx.x * R + step - 1) / step;
+    const float inv_n = 1.0f / (float)N;
+    if (L == kBlock) {
+        if (threadIdx.x < 64) red[threadIdx.x >> 4][threadIdx.x & 15] = 0.0f;
+        __syncthreads();
+    }
+    float wv[C][8], aw[C][8], ab[C][8];
+    Raw8<DT> rx[C], rg[C];
+    float mean, rstd;
+    auto load = [&](int64_t at) {
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            const int c = (k * lanes + l) * 8;
+            rx[k] = load_piece<DT, RAGGED>(elem_at<DT>(x, at * x_pitch), c, N, at < M);
+            rg[k] = load_piece<DT, RAGGED>(elem_at<DT>(dy, at * dy_pitch), c, N, at < M);
+        }
+        mean = at < M ? mean_in[at] : 0.0f;
+        rstd = at < M ? rstd_in[at] : 0.0f;
+    };
+    if (!kLean) load(row);
+#pragma unroll
+    for (int k = 0; k < C; k++) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            wv[k][j] = 1.0f;
+            aw[k][j] = ab[k][j] = 0.0f;
+        }
+        if (w) load8_rt(w, w_dt, (k * lanes + l) * 8, N, wv[k]);
+    }
+    for (int64_t i = 0; i < rounds; i++, row += step) {
+        if (kLean) load(row);
+        float h[C][8], t[C][8], st = 0.0f, sth = 0.0f;
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            if (RAGGED) {
+                settle_row8<DT>(rx[k], (k * lanes + l) * 8, N);
+                settle_row8<DT>(rg[k], (k * lanes + l) * 8, N);  // zeros past the end: they add nothing to any sum
+            }
+            raw8_to_f32<DT>(rx[k], h[k]);
+            raw8_to_f32<DT>(rg[k], t[k]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                h[k][j] = (h[k][j] - mean) * rstd;
+                if (SUMS) {
+                    aw[k][j] = fmaf(t[k][j], h[k][j], aw[k][j]);
+                    ab[k][j] += t[k][j];
+                }
+                t[k][j] *= wv[k][j];
+                st += t[k][j];
+                sth = fmaf(t[k][j], h[k][j], sth);
+            }
+        }
+        const float rs = rstd;
+        if (!kLean && i + 1 < rounds) load(row + step);
+        if (dx) {
+            float mt, mth;
+            if (L != kBlock) {
+                mt = row_sum<L>(st, nullptr) * inv_n;
+                mth = row_sum<L>(sth, nullptr) * inv_n;
+            } else {  // both sums behind one barrier; the buffers alternate from row to row
+                st = cluster_sum<64>(st);
+                sth = cluster_sum<64>(sth);
+                float *ra = red[2 * (i & 1)], *rb = red[2 * (i & 1) + 1];
+                if ((threadIdx.x & 63) == 0) {
+                    ra[threadIdx.x >> 6] = st;
+                    rb[threadIdx.x >> 6] = sth;
+                }
+                __syncthreads();
+                mt = cluster_sum<16>(ra[threadIdx.x & 15]) * inv_n;
+                mth = cluster_sum<16>(rb[threadIdx.x & 15]) * inv_n;
+            }
+            if (row < M) {
+#pragma unroll
+                for (int k = 0; k < C; k++) {
+                    const int c = (k * lanes + l) * 8;
+                    if (c >= N) continue;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) t[k][j] = (t[k][j] - fmaf(h[k][j], mth, mt)) * rs;
+                    store8<DT>(elem_at<DT>(dx, row * N + c), RAGGED ? N - c : 8, t[k]);
+                }
+            }
+        }
+    }
+    if (SUMS) {
+        if (!kShared) {
+#pragma unroll
+            for (int k = 0; k < C; k++) {
+                const int c = (k * lanes + l) * 8;
+                if (pw) store8<kF32>(pw + blockIdx.x * (int64_t)N + c, N - c, aw[k]);
+                if (pb) store8<kF32>(pb + blockIdx.x * (int64_t)N + c, N - c, ab[k]);
+            }
+        } else {
+#pragma unroll
+            for (int which = 0; which < 2; which++) {
+                float* out = which == 0 ? pw : pb;
+                if (!out) continue;
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < C; k++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) cols[kShared ? r : 0][kShared ? (k * L + l) * 8 + j : 0] = which == 0 ? aw[k][j] : ab[k][j];
+                __syncthreads();
+                for (int c = threadIdx.x; c < N; c += 256) {
+                    float s = cols[0][kShared ? c : 0];
+                    for (int k = 1; k < R; k++) s += cols[kShared ? k : 0][kShared ? c : 0];
+                    out[blockIdx.x * (int64_t)N + c] = s;
+                }
+            }
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ rows of any length
@@ -138,9 +371,10 @@ __global__ __launch_bounds__(256) void k_ln_bwd_wb_long(const void* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------------ dw, db from partial rows
-// 32 columns a block (one 128-byte line of each partial row); 16 slices of threads take the rows in turn, slice sums are
-// added in slice order.  blockIdx.y: 0 = the first pair given, 1 = the second.
-constexpr int kSumCols = 32, kSumSlices = 16;
+// 32 columns a block (one 128-byte line of each partial row); 32 slices of threads take the rows in turn, eight loads in flight
+// each (one load at a time took 15 us more at 512 x 4096); slice sums are added in slice order.  blockIdx.y: 0 = the first pair
+// given, 1 = the second.
+constexpr int kSumCols = 32, kSumSlices = 32;
 __global__ __launch_bounds__(kSumCols* kSumSlices) void k_ln_sum_partials(const float* __restrict__ pw, void* __restrict__ dw,
                                                                          const float* __restrict__ pb, void* __restrict__ db, int dt,
                                                                          int64_t rows, int64_t N) {
@@ -151,7 +385,15 @@ __global__ __launch_bounds__(kSumCols* kSumSlices) void k_ln_sum_partials(const 
     void* out = blockIdx.y == 0 && dw ? dw : db;
     float s = 0.0f;
     if (c < N)
-        for (int64_t r = slice; r < rows; r += kSumSlices) s += p[r * N + c];
+        for (int64_t r0 = slice; r0 < rows; r0 += kSumSlices * 8) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int64_t r = r0 + k * kSumSlices;
+                v[k] = r < rows ? p[r * N + c] : 0.0f;
+            }
+            s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        }
     red[slice][col] = s;
     __syncthreads();
     if (slice == 0 && c < N) {
@@ -171,6 +413,57 @@ using namespace coat;
 static bool ln_dtype(int dt) { return dt == COAT_F32 || dt == COAT_BF16 || dt == COAT_F16; }
 static bool ln_aligned(const void* p, int dt) { return ((uintptr_t)p & (dt == COAT_F32 ? 3u : 1u)) == 0; }
 
+// How rows of N elements are held in registers: threads of a block, rows it works on at a time; threads 0: they are not.
+struct LnShape {
+    int threads, rows;
+};
+// sums: the kernel that also sums dw and db, which takes the longest rows with 512 threads: their sums, weights and values would
+// not fit into the 128 registers that each of 1024 threads has.
+static LnShape ln_shape(int64_t N, bool sums) {
+    if (N <= 512) return {256, N <= 64 ? 32 : N <= 128 ? 16 : N <= 256 ? 8 : 4};
+    if (N <= 8192) return {(int)((N + 511) / 512) * 64, 1};
+    if (N <= 16384) return {sums ? (int)((N + 2047) / 2048) * 64 : (int)((N + 1023) / 1024) * 64, 1};
+    return {0, 1};
+}
+// Calls f(L, C, RAGGED) (as integral constants) for that form.
+template <bool SUMS, typename F> static void ln_form(int64_t N, F f) {
+#define FORM(LANES, PIECES)                                                                                                      \
+    if (N % 8) f(std::integral_constant<int, LANES>(), std::integral_constant<int, PIECES>(), std::integral_constant<bool, true>()); \
+    else f(std::integral_constant<int, LANES>(), std::integral_constant<int, PIECES>(), std::integral_constant<bool, false>())
+    if (N <= 64) { FORM(8, 1); }
+    else if (N <= 128) { FORM(16, 1); }
+    else if (N <= 256) { FORM(32, 1); }
+    else if (N <= 512) { FORM(64, 1); }
+    else if (N <= 8192) { FORM(kBlock, 1); }
+    else { FORM(kBlock, (SUMS ? 4 : 2)); }
+#undef FORM
+}
+static int64_t ln_rounds(int64_t M, int64_t N) {
+    const int rows = ln_shape(N, true).rows;
+    return (M + rows - 1) / rows;
+}
+// Blocks of a kernel that only streams: 2^20 threads.
+static unsigned ln_blocks(int64_t M, int64_t N, int threads) {
+    const int64_t rounds = ln_rounds(M, N), most = (1 << 20) / threads;
+    return (unsigned)(rounds < most ? rounds : most);
+}
+
+template <int DT>
+static int ln_forward(const void* x, int64_t x_pitch, const void* w, const void* b, int w_dtype, void* y, float* mean, float* rstd,
+                      int64_t M, int64_t N, float eps, hipStream_t st) {
+    const LnShape shape = ln_shape(N, false);
+    if (shape.threads)
+        ln_form<false>(N, [&](auto lanes, auto pieces, auto ragged) {
+            hipLaunchKernelGGL((k_ln_fwd<DT, decltype(lanes)::value, decltype(pieces)::value, decltype(ragged)::value>),
+                               dim3(ln_blocks(M, N, shape.threads)), dim3(shape.threads), 0, st, x, x_pitch, w, b, w_dtype, y, mean, rstd, M,
+                               (int)N, eps);
+        });
+    else
+        hipLaunchKernelGGL((k_ln_fwd_long<DT>), dim3((unsigned)(M < 65536 ? M : 65536)), dim3(256), 0, st, x, x_pitch, w, b, w_dtype, y, mean,
+                           rstd, M, N, eps);
+    return coat_launch_status();
+}
+
 extern "C" int coat_layer_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const void* w, const void* b, int w_dtype,
                                        void* y, float* mean, float* rstd, int64_t M, int64_t N, float eps, void* stream) {
     if (!ln_dtype(x_dtype) || (w && !ln_dtype(w_dtype))) return COAT_EDTYPE;
@@ -182,27 +475,46 @@ extern "C" int coat_layer_norm_forward(const void* x, int64_t x_pitch, int x_dty
     if (!ln_aligned(x, x_dtype) || !ln_aligned(y, x_dtype) || !ln_aligned(mean, COAT_F32) || !ln_aligned(rstd, COAT_F32) ||
         (w && !ln_aligned(w, w_dtype)) || (b && !ln_aligned(b, w_dtype)))
         return COAT_EALIGN;
-    const dim3 grid((unsigned)(M < 65536 ? M : 65536));
     hipStream_t st = (hipStream_t)stream;
-    if (x_dtype == COAT_F32)
-        hipLaunchKernelGGL((k_ln_fwd_long<kF32>), grid, dim3(256), 0, st, x, x_pitch, w, b, w_dtype, y, mean, rstd, M, N, eps);
-    else if (x_dtype == COAT_BF16)
-        hipLaunchKernelGGL((k_ln_fwd_long<kBF16>), grid, dim3(256), 0, st, x, x_pitch, w, b, w_dtype, y, mean, rstd, M, N, eps);
-    else
-        hipLaunchKernelGGL((k_ln_fwd_long<kF16>), grid, dim3(256), 0, st, x, x_pitch, w, b, w_dtype, y, mean, rstd, M, N, eps);
-    return coat_launch_status();
+    switch (x_dtype) {
+        case COAT_F32: return ln_forward<kF32>(x, x_pitch, w, b, w_dtype, y, mean, rstd, M, N, eps, st);
+        case COAT_BF16: return ln_forward<kBF16>(x, x_pitch, w, b, w_dtype, y, mean, rstd, M, N, eps, st);
+        default: return ln_forward<kF16>(x, x_pitch, w, b, w_dtype, y, mean, rstd, M, N, eps, st);
+    }
 }
 
 extern "C" int coat_layer_norm_partials(int64_t M, int64_t N) {
     if (M < 0 || N <= 0) return COAT_EINVAL;
-    return (int)(M < 256 ? (M > 0 ? M : 1) : 256);
+    // As many blocks as keep the memory busy: 256 of 512 threads and more, up to 1024 of fewer threads, whole numbers a CU (8192 x
+    // 4096 bf16: 41 us with 256, 43 with 384, 49 with 1024).  With few rows, fewer: a partial row costs as much to write and to
+    // sum as it saves (1024 x 4096 bf16: 14 us with 192, 23 with 1024; the factor is fitted to such sweeps).
+    const int threads = ln_shape(N, true).threads ? ln_shape(N, true).threads : 256;
+    const int64_t rounds = ln_rounds(M, N), per_cu = N > 8192 || threads > 960 ? 1 : 960 / threads > 4 ? 4 : 960 / threads, most = 256 * per_cu;
+    const double balanced = sqrt(27.0 * (double)rounds * (N < 4096 ? 4096.0 / (double)N : 1.0));
+    int64_t n = balanced < (double)most ? (int64_t)balanced : most;
+    if (n > rounds) n = rounds;
+    return (int)(n < 1 ? 1 : n);
 }
 
 template <int DT>
 static int ln_backward(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, const float* mean, const float* rstd,
                        const void* w, int w_dtype, void* dx, void* dw, void* db, int wb_dtype, float* pw, float* pb, int n_partial,
                        int64_t M, int64_t N, hipStream_t st) {
-    if (M > 0) {
+    if (n_partial > ln_rounds(M, N)) n_partial = (int)ln_rounds(M, N);
+    const bool sums = dw || db;
+    const LnShape shape = ln_shape(N, sums);
+    if (M > 0 && shape.threads) {
+#define BACKWARD(SUMS, BLOCKS)                                                                                                           \
+    ln_form<SUMS>(N, [&](auto lanes, auto pieces, auto ragged) {                                                                         \
+        hipLaunchKernelGGL((k_ln_bwd<DT, decltype(lanes)::value, decltype(pieces)::value, decltype(ragged)::value, SUMS>), dim3(BLOCKS), \
+                           dim3(shape.threads), 0, st, dy, dy_pitch, x, x_pitch, mean, rstd, w, w_dtype, dx, dw ? pw : nullptr,          \
+                           db ? pb : nullptr, M, (int)N);                                                                                \
+    })
+        if (sums) BACKWARD(true, (unsigned)n_partial);
+        else BACKWARD(false, ln_blocks(M, N, shape.threads));
+#undef BACKWARD
+        if (const int rc = coat_launch_status()) return rc;
+    } else if (M > 0) {
         if (dx) {
             hipLaunchKernelGGL((k_ln_bwd_long<DT>), dim3((unsigned)(M < 65536 ? M : 65536)), dim3(256), 0, st, dy, dy_pitch, x, x_pitch, mean,
                                rstd, w, w_dtype, dx, M, N);
