@@ -20,14 +20,20 @@ def _rows(t, N):
     return t, t.stride(0) if t.shape[0] > 1 else N
 
 
+def _dense_like(t):
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _check(who, x, weight, bias):
     if not x.is_cuda:
         raise RuntimeError("coat_amd kernels need tensors on the GPU (got a %s tensor)" % x.device.type)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{who}: expected a tensor with a last dimension to normalise over, got shape {tuple(x.shape)}")
     _hip.dt(x)
-    if bias is not None and weight is None:
-        raise ValueError(f"{who}: a bias needs a weight")
+    if weight is None:
+        if bias is not None:
+            raise ValueError(f"{who}: a bias needs a weight")
+        return
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
@@ -47,13 +53,13 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
     if not eps >= 0.0:
         raise ValueError(f"layer_norm_forward: invalid eps {eps}")
     N = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     rstd = torch.empty_like(mean)
     x, pitch = _rows(x, N)
     w = weight if weight is None else weight.contiguous()
     b = bias if bias is None else bias.contiguous()
-    _hip.launch("coat_layer_norm_forward", x.device, x.data_ptr(), pitch, _hip.dt(x), None if w is None else w.data_ptr(),
+    _hip.launch("coat_layer_norm_forward", x.get_device(), x.data_ptr(), pitch, _hip.dt(x), None if w is None else w.data_ptr(),
                 None if b is None else b.data_ptr(), 0 if w is None else _hip.dt(w), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
                 x.shape[0], N, float(eps), what="layer_norm_forward")
     return y, mean, rstd
@@ -71,9 +77,9 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, bias_grad=True, *, x_gra
         if t.dtype != torch.float32 or t.numel() != M or t.device != device or not t.is_contiguous():
             raise ValueError(f"layer_norm_backward: {name} must be contiguous fp32 with one element a row, on x's device")
     w = weight if weight is None else weight.contiguous()
-    dx = torch.empty(shape, dtype=x.dtype, device=device) if x_grad else None
-    dw = torch.empty((N,), dtype=w.dtype, device=device) if w is not None and weight_grad else None
-    db = torch.empty((N,), dtype=w.dtype, device=device) if w is not None and bias_grad else None
+    dx = _dense_like(x) if x_grad else None
+    dw = torch.empty_like(w) if w is not None and weight_grad else None
+    db = torch.empty_like(w) if w is not None and bias_grad else None
     parts, partial = 0, None
     wanted = (dw is not None) + (db is not None)
     if wanted:
@@ -83,7 +89,7 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, bias_grad=True, *, x_gra
         partial = torch.empty((wanted, parts, N), dtype=torch.float32, device=device)
     x, x_pitch = _rows(x, N)
     dy, dy_pitch = _rows(dy, N)
-    _hip.launch("coat_layer_norm_backward", device, dy.data_ptr(), dy_pitch, x.data_ptr(), x_pitch, _hip.dt(x), mean.data_ptr(),
+    _hip.launch("coat_layer_norm_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x_pitch, _hip.dt(x), mean.data_ptr(),
                 rstd.data_ptr(), None if w is None else w.data_ptr(), 0 if w is None else _hip.dt(w),
                 *(None if t is None else t.data_ptr() for t in (dx, dw, db, partial)), parts, M, N, what="layer_norm_backward")
     return dx, dw, db

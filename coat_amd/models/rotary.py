@@ -26,7 +26,7 @@ class RotaryAxes:
             raise ValueError(f"RotaryAxes: sections {self.sections} hold more pairs than a head of {self.head_dim}")
         if not (self.theta > 0.0 and math.isfinite(self.theta)):
             raise ValueError(f"RotaryAxes: invalid theta {theta}")
-        total = sum(self.sections)
+        total = self.turning = sum(self.sections)  # P
         self._axis = [a for a, n in enumerate(self.sections) for _ in range(n)]
         exponent = [i / n for n in self.sections for i in range(n)] if self.restart else [j / total for j in range(total)]
         self._freq = [self.theta ** -e for e in exponent]  # radians a position, in 64 bits
@@ -58,7 +58,7 @@ def _positions(position_ids, plan, B, S, device):
         if position_ids.dtype.is_floating_point or position_ids.dtype.is_complex or position_ids.dtype == torch.bool:
             raise ValueError(f"rotary_axes: position_ids must be whole numbers, got {position_ids.dtype}")
         position_ids = position_ids.long()
-    return position_ids.expand(-1, B, S)
+    return position_ids if position_ids.shape[1:] == (B, S) else position_ids.expand(-1, B, S)
 
 
 def _rotate(q, k, position_ids, plan, inverse):
@@ -80,17 +80,17 @@ def _rotate(q, k, position_ids, plan, inverse):
     args, outs, kept = [], [], []
     for t in (q, k):
         if t is None:
-            args += [None, None, 0, 0, 0, 0]
+            args += (None, None, 0, 0, 0, 0)
             outs.append(None)
             continue
-        if t.stride(3) != 1 and D > 1:
+        if t.stride(3) != 1:
             t = t.contiguous()
         kept.append(t)
-        out = torch.empty(t.shape, dtype=t.dtype, device=device)
-        args += [t.data_ptr(), out.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2]]
+        out = torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=device)
         outs.append(out)
-    _hip.launch("coat_rope_axes", device, *args, _hip.dt(first), pos.data_ptr(), *pos.stride(), len(plan.sections), turns.data_ptr(),
-                axis.data_ptr(), sum(plan.sections), D, 1 if plan.pairs else 0, 1 if inverse else 0, B, S, what="rotary_axes")
+        args += (t.data_ptr(), out.data_ptr(), *t.stride()[:3], t.shape[2])
+    _hip.launch("coat_rope_axes", first.get_device(), *args, _hip.dt(first), pos.data_ptr(), *pos.stride(), len(plan.sections),
+                turns.data_ptr(), axis.data_ptr(), plan.turning, D, plan.pairs, inverse, B, S, what="rotary_axes")
     return outs[0], outs[1]
 
 

@@ -8,6 +8,7 @@ torch tensors in, everything updated in place; the work is done by libcoat_hip.s
 stream (the reference launches on the legacy default stream).  Errors the reference raises through
 AT_ASSERTM surface as RuntimeError with the same message."""
 import ctypes
+from array import array
 
 import torch
 
@@ -120,26 +121,30 @@ def fp8_adamw_step_multi(params, grads, exp_avg, scale_exp_avg, exp_avg_sq, scal
 
 # ------------------------------------------------------------------------------------------------ 32-bit states, clipping
 def _columns(what, lists):
-    """Checks parallel lists of tensors (name, tensors, dtypes allowed or None) that a multi-tensor call reads or writes flat: one
-    length, one device, one dtype a list, equal sizes, contiguous.  Returns (device, sizes, addresses of each list)."""
+    """Checks parallel lists of tensors (name, tensors, dtype of all or None) that a multi-tensor call reads or writes flat: one
+    length, one device, equal sizes, contiguous.  Returns (device index, sizes, addresses of each list)."""
     first = lists[0][1]
-    n, index = len(first), first[0].get_device()
+    n, index, T = len(first), first[0].get_device(), torch.Tensor
     if index < 0:
         raise RuntimeError(f"{what}: tensors must be on the GPU")
-    numel, out = list(map(torch.Tensor.numel, first)), []
+    numel, out = list(map(T.numel, first)), []
     for name, tensors, dtype in lists:
         if len(tensors) != n:
             raise RuntimeError(f"{what}: the tensor lists differ in length")
-        if set(map(torch.Tensor.get_device, tensors)) != {index}:
+        if set(map(T.get_device, tensors)) != {index}:
             raise RuntimeError(f"{what}: {name} holds tensors that are not on the first tensor's device")
         if dtype is not None and {t.dtype for t in tensors} != {dtype}:
             raise RuntimeError(f"{what}: {name} must all be {dtype}")
-        if list(map(torch.Tensor.numel, tensors)) != numel:
+        if tensors is not first and list(map(T.numel, tensors)) != numel:
             raise RuntimeError(f"{what}: sizes of {name} differ from those of {lists[0][0]}")
-        if not all(map(torch.Tensor.is_contiguous, tensors)):
+        if not all(map(T.is_contiguous, tensors)):
             raise RuntimeError(f"{what}: {name} must be contiguous")
-        out.append(list(map(torch.Tensor.data_ptr, tensors)))
-    return first[0].device, numel, out
+        out.append(list(map(T.data_ptr, tensors)))
+    return index, numel, out
+
+
+def _address(host_array):
+    return host_array.buffer_info()[0]
 
 
 def grad_norm_multi(grads, max_norm=None):
@@ -154,17 +159,20 @@ def grad_norm_multi(grads, max_norm=None):
         raise ValueError(f"grad_norm_multi: invalid max_norm {max_norm}")
     if not grads:
         raise ValueError("grad_norm_multi: no gradients")
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
+    if not all(map(torch.Tensor.is_contiguous, grads)):
+        grads = [g.contiguous() for g in grads]
     n = len(grads)
-    device, numel, (addresses,) = _columns("grad_norm_multi", [("grads", grads, None)])
-    dtypes = (ctypes.c_int * n)(*[_hip.dt(g) for g in grads])
-    numel = (ctypes.c_int64 * n)(*numel)
-    parts = _hip.lib().coat_grad_norm_partials(n, numel)
+    index, numel, (addresses,) = _columns("grad_norm_multi", [("grads", grads, None)])
+    kinds = {g.dtype for g in grads}
+    dtypes = array("i", [_hip.dt(k) for k in kinds] * n if len(kinds) == 1 else [_hip.dt(g) for g in grads])
+    numel, addresses = array("q", numel), array("Q", addresses)
+    parts = _hip.lib().coat_grad_norm_partials(n, _address(numel))
     if parts < 0:
         _hip.check(parts, "grad_norm_multi")
+    device = grads[0].device
     work = torch.empty(max(parts, 1), dtype=torch.float64, device=device)
     out = torch.empty(2, dtype=torch.float32, device=device)
-    _hip.launch("coat_grad_norm_multi", device, n, (ctypes.c_void_p * n)(*addresses), dtypes, numel,
+    _hip.launch("coat_grad_norm_multi", index, n, _address(addresses), _address(dtypes), _address(numel),
                 0.0 if max_norm is None else float(max_norm), work.data_ptr(), parts, out.data_ptr(), what="grad_norm_multi")
     norm, scale = out.unbind()
     return norm, None if max_norm is None else scale
@@ -182,22 +190,29 @@ def adamw_step_multi(params, grads, exp_avg, exp_avg_sq, beta1, beta2, lr, wd, e
              ("exp_avg", exp_avg, torch.float32), ("exp_avg_sq", exp_avg_sq, torch.float32)]
     if masters is not None:
         lists.append(("masters", masters, torch.float32))
-    device, numel, addresses = _columns("adamw_step_multi", lists)
+    index, numel, addresses = _columns("adamw_step_multi", lists)
     pdt, gdt = params[0].dtype, grads[0].dtype
     if gdt != pdt and gdt != torch.float32:
         raise RuntimeError(f"adamw_step_multi: grads dtype {gdt} is neither the params' {pdt} nor torch.float32")
     if masters is not None and pdt == torch.float32:
         raise RuntimeError("adamw_step_multi: masters are for parameters of 16 bits")
-    written = [a for column in addresses[:1] + addresses[2:] for a, size in zip(column, numel) if size]
-    if len(set(written)) != len(written):
-        raise RuntimeError("adamw_step_multi: a tensor that is stepped is given twice")
+    written = addresses[0] + [a for column in addresses[2:] for a in column]
+    if len(set(written)) != len(written):  # empty tensors share the address 0
+        sizes = numel * (len(addresses) - 1)
+        written = [a for a, size in zip(written, sizes) if size]
+        if len(set(written)) != len(written):
+            raise RuntimeError("adamw_step_multi: a tensor that is stepped is given twice")
     if not int(step) >= 1:
         raise ValueError(f"adamw_step_multi: invalid step {step}")
-    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != device):
+    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.get_device() != index):
         raise RuntimeError("adamw_step_multi: grad_scale must be one fp32 element on the parameters' device")
-    arrays = [(ctypes.c_void_p * n)(*a) for a in addresses]
-    _hip.launch("coat_adamw_step_multi", device, n, arrays[0], _hip.dt(pdt), arrays[1], _hip.dt(gdt), arrays[2], arrays[3],
-                arrays[4] if masters is not None else None, (ctypes.c_int64 * n)(*numel), (ctypes.c_double * 5)(beta1, beta2, lr, wd, eps),
-                int(step), None if grad_scale is None else grad_scale.data_ptr(), what="adamw_step_multi")
+    arrays = [array("Q", a) for a in addresses]
+    numel, hyper = array("q", numel), array("d", (beta1, beta2, lr, wd, eps))
+    _hip.launch("coat_adamw_step_multi", index, n, _address(arrays[0]), _hip.dt(pdt), _address(arrays[1]), _hip.dt(gdt),
+                _address(arrays[2]), _address(arrays[3]), _address(arrays[4]) if masters is not None else None, _address(numel),
+                _address(hyper), int(step), None if grad_scale is None else grad_scale.data_ptr(), what="adamw_step_multi")
     # written behind autograd's back: graphs that saved them must notice
-    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+    try:
+        torch.autograd.graph.increment_version(params)
+    except RuntimeError:  # inference tensors have no version
+        torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
