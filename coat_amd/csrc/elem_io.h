@@ -68,6 +68,15 @@ template <int DT> __device__ __forceinline__ Raw8<DT> load_row8(const void* row,
     }
     return r;
 }
+// RAGGED: n need not be a multiple of 8.  Otherwise c is below n only where a whole piece is.
+template <int DT, bool RAGGED> __device__ __forceinline__ Raw8<DT> load_piece(const void* row, int c, int n, bool valid = true) {
+    if (RAGGED) return load_row8<DT>(row, c, n, valid);
+    Raw8<DT> r;
+#pragma unroll
+    for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = 0;
+    if (valid && c < n) r = load_raw8<DT>(elem_at<DT>(row, c), 8);
+    return r;
+}
 template <int DT> __device__ __forceinline__ void settle_row8(Raw8<DT>& r, int c, int n) {
     const int past = c + 8 - n;  // elements of this piece past the end of the row
     if (past > 0 && past < 8 && n >= 8) {

@@ -48,15 +48,6 @@ template <int L> __device__ __forceinline__ float row_sum(float v, float* red) {
     __syncthreads();
     return cluster_sum<16>(red[threadIdx.x & 15]);
 }
-template <int DT, bool RAGGED> __device__ __forceinline__ Raw8<DT> load_piece(const void* row, int c, int N, bool valid) {
-    if (RAGGED) return load_row8<DT>(row, c, N, valid);
-    Raw8<DT> r;
-#pragma unroll
-    for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = 0;
-    if (valid && c < N) r = load_raw8<DT>(elem_at<DT>(row, c), 8);
-    return r;
-}
-
 template <int DT, int L, int C, bool RAGGED>
 __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __restrict__ x, int64_t x_pitch, const void* __restrict__ w,
                                                                  const void* __restrict__ b, int w_dt, void* __restrict__ y,

@@ -34,16 +34,53 @@ struct RopeArgs {
     const int32_t* axis;
     int64_t tokens, seq;
     int axes, head_dim, pairs, per_block;  // per_block: tokens a block takes at a time
+    uint32_t magic_pieces, magic_heads, magic_pairs;
     float sign;
 };
 
-template <int DT, bool ADJ>
+// n / d for n * d < 2^32, with m = ceil(2^32 / d)
+__device__ __forceinline__ uint32_t div_magic(uint32_t n, uint32_t d, uint32_t m) { return d == 1 ? n : __umulhi(n, m); }
+
+// WHOLE: every piece is complete (pairs and head_dim multiples of 8), no element-wise ends.
+template <int DT, bool ADJ, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rope_axes(RopeArgs A) {
     __shared__ float2 cs[kRopeSlots];
     const int64_t first = (int64_t)blockIdx.x * A.per_block;
     const int here = (int)(A.tokens - first < A.per_block ? A.tokens - first : A.per_block);
+    // a job is one 8-element piece: of the first halves together with the same piece of the second halves, of adjacent pairs,
+    // or of the rest behind the pairs
+    const int rot = 2 * A.pairs, heads = A.q.heads + A.k.heads;
+    const int turning = ((ADJ ? rot : A.pairs) + 7) >> 3, pieces = turning + ((A.head_dim - rot + 7) >> 3);
+    const int jobs = here * heads * pieces;
+    struct Job {
+        Raw8<DT> a, b;
+        void* y;
+        int piece, token, e, n;
+    };
+    auto fetch = [&](int job) {
+        Job J;
+        const uint32_t th = div_magic(job, pieces, A.magic_pieces);
+        J.piece = job - (int)th * pieces;
+        J.token = div_magic(th, heads, A.magic_heads);
+        int head = (int)th - J.token * heads;
+        const int64_t token = first + J.token, b = token / A.seq, s = token - b * A.seq;
+        const bool is_k = head >= A.q.heads;
+        if (is_k) head -= A.q.heads;
+        const void* x = is_k ? elem_at<DT>(A.k.x, b * A.k.sb + s * A.k.ss + head * A.k.sh)
+                             : elem_at<DT>(A.q.x, b * A.q.sb + s * A.q.ss + head * A.q.sh);
+        J.y = is_k ? elem_at<DT>(A.k.y, (token * A.k.heads + head) * A.head_dim) : elem_at<DT>(A.q.y, (token * A.q.heads + head) * A.head_dim);
+        // the run of elements that the piece belongs to (all pairs, the first and second halves, or the rest), and its place there
+        const bool rest = J.piece >= turning;
+        J.e = (rest ? J.piece - turning : J.piece) * 8;
+        J.n = rest ? A.head_dim - rot : ADJ ? rot : A.pairs;
+        J.a = load_piece<DT, !WHOLE>(rest ? elem_at<DT>(x, rot) : x, J.e, J.n);
+        if (!ADJ && !rest) J.b = load_piece<DT, !WHOLE>(elem_at<DT>(x, A.pairs), J.e, J.n);
+        return J;
+    };
+    Job J;
+    if ((int)threadIdx.x < jobs) J = fetch(threadIdx.x);  // in flight while the sines are computed
     for (int i = threadIdx.x; i < here * A.pairs; i += 256) {
-        const int t = i / A.pairs, j = i - t * A.pairs;
+        const int t = div_magic(i, A.pairs, A.magic_pairs), j = i - t * A.pairs;
         const int64_t token = first + t, b = token / A.seq, s = token - b * A.seq;
         const int a = min(max(A.axis[j], 0), A.axes - 1);
         const double turns = (double)A.pos[a * A.pos_sa + b * A.pos_sb + s * A.pos_ss] * A.turns[j];
@@ -52,48 +89,39 @@ __global__ __launch_bounds__(256) void k_rope_axes(RopeArgs A) {
         cs[i] = make_float2(c, A.sign * sn);
     }
     __syncthreads();
-    // a job is one 8-element piece: of the first halves together with the same piece of the second halves, of adjacent pairs,
-    // or of the rest behind the pairs
-    const int rot = 2 * A.pairs, heads = A.q.heads + A.k.heads;
-    const int turning = ((ADJ ? rot : A.pairs) + 7) >> 3, pieces = turning + ((A.head_dim - rot + 7) >> 3);
-    const int jobs = here * heads * pieces;
-    for (int job = threadIdx.x; job < jobs; job += 256) {
-        const int th = job / pieces, piece = job - th * pieces, t = th / heads;
-        int head = th - t * heads;
-        const int64_t token = first + t, b = token / A.seq, s = token - b * A.seq;
-        const bool is_k = head >= A.q.heads;
-        const RopeTensor& T = is_k ? A.k : A.q;
-        if (is_k) head -= A.q.heads;
-        const void* x = elem_at<DT>(T.x, b * T.sb + s * T.ss + head * T.sh);
-        void* y = elem_at<DT>(T.y, (token * T.heads + head) * A.head_dim);
+    for (int job = threadIdx.x; job < jobs;) {
+        const int e = J.e, left = WHOLE ? 8 : J.n - e, piece = J.piece;
+        void* y = J.y;
+        const float2* c = cs + J.token * A.pairs;
         float u[8], v[8];
+        if (!WHOLE) {
+            settle_row8<DT>(J.a, e, J.n);
+            if (!ADJ) settle_row8<DT>(J.b, e, J.n);
+        }
+        raw8_to_f32<DT>(J.a, u);
+        if (!ADJ) raw8_to_f32<DT>(J.b, v);
+        job += 256;
+        if (job < jobs) J = fetch(job);
         if (piece >= turning) {
-            const int e = rot + (piece - turning) * 8;
-            load8<DT>(elem_at<DT>(x, e), A.head_dim - e, u);
-            store8<DT>(elem_at<DT>(y, e), A.head_dim - e, u);
+            store8<DT>(elem_at<DT>(y, rot + e), left, u);
         } else if (ADJ) {
-            const int e = piece * 8;
-            load8<DT>(elem_at<DT>(x, e), rot - e, u);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float2 c = cs[t * A.pairs + min((e >> 1) + i, A.pairs - 1)];
-                v[2 * i] = u[2 * i] * c.x - u[2 * i + 1] * c.y;
-                v[2 * i + 1] = u[2 * i + 1] * c.x + u[2 * i] * c.y;
+                const float2 f = c[WHOLE ? (e >> 1) + i : min((e >> 1) + i, A.pairs - 1)];
+                v[2 * i] = u[2 * i] * f.x - u[2 * i + 1] * f.y;
+                v[2 * i + 1] = u[2 * i + 1] * f.x + u[2 * i] * f.y;
             }
-            store8<DT>(elem_at<DT>(y, e), rot - e, v);
+            store8<DT>(elem_at<DT>(y, e), left, v);
         } else {
-            const int e = piece * 8;
-            load8<DT>(elem_at<DT>(x, e), A.pairs - e, u);
-            load8<DT>(elem_at<DT>(x, e + A.pairs), A.pairs - e, v);
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                const float2 c = cs[t * A.pairs + min(e + i, A.pairs - 1)];
+                const float2 f = c[WHOLE ? e + i : min(e + i, A.pairs - 1)];
                 const float x1 = u[i], x2 = v[i];
-                u[i] = x1 * c.x - x2 * c.y;
-                v[i] = x2 * c.x + x1 * c.y;
+                u[i] = x1 * f.x - x2 * f.y;
+                v[i] = x2 * f.x + x1 * f.y;
             }
-            store8<DT>(elem_at<DT>(y, e), A.pairs - e, u);
-            store8<DT>(elem_at<DT>(y, e + A.pairs), A.pairs - e, v);
+            store8<DT>(elem_at<DT>(y, e), left, u);
+            store8<DT>(elem_at<DT>(y, e + A.pairs), left, v);
         }
     }
 }
@@ -110,7 +138,7 @@ extern "C" int coat_rope_axes(const void* q, void* q_out, int64_t q_sb, int64_t 
     if (batch < 0 || seq < 0 || q_heads < 0 || k_heads < 0 || axes < 1 || pairs < 1 || head_dim < 2 || adjacent < 0 || adjacent > 1 ||
         inverse < 0 || inverse > 1)
         return COAT_EINVAL;
-    if (2 * (int64_t)pairs > head_dim || q_heads > 4096 || k_heads > 4096 || head_dim > 2 * kRopeSlots) return COAT_ESHAPE;
+    if (2 * (int64_t)pairs > head_dim || q_heads > 1024 || k_heads > 1024 || head_dim > 2 * kRopeSlots) return COAT_ESHAPE;
     if (batch == 0 || seq == 0 || q_heads + k_heads == 0) return COAT_OK;
     if ((q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)) || !pos || !turns || !axis) return COAT_EINVAL;
     const uintptr_t mask = dtype == COAT_F32 ? 3 : 1;
@@ -128,16 +156,28 @@ extern "C" int coat_rope_axes(const void* q, void* q_out, int64_t q_sb, int64_t 
     A.seq = seq;
     A.axes = axes; A.head_dim = head_dim; A.pairs = pairs;
     A.sign = inverse ? -1.0f : 1.0f;
-    int per = 4;
-    while (per > 1 && per * pairs > kRopeSlots) per >>= 1;
+    const int turning = ((adjacent ? 2 * pairs : pairs) + 7) / 8, pieces = turning + (head_dim - 2 * pairs + 7) / 8;
+    auto magic = [](int d) { return (uint32_t)((((uint64_t)1 << 32) + d - 1) / d); };
+    A.magic_pieces = magic(pieces);
+    A.magic_heads = magic(q_heads + k_heads);
+    A.magic_pairs = magic(pairs);
+    const bool whole = head_dim % 8 == 0 && (adjacent ? pairs % 4 == 0 : pairs % 8 == 0);
+    // about 512 pieces a block: two rounds of its 256 threads, the second in flight under the first, next to the sines of as few
+    // tokens as possible (bf16, 4 x 2048 tokens, 64 heads of 128: one token 46 us, four 48, sixteen 69; 4 x 4096 tokens, 16 heads
+    // of 64: one 22 us, eight 13); fewer where the tokens are too few to fill the card.
+    const int64_t per_token = (int64_t)(q_heads + k_heads) * pieces;
+    int per = 1;
+    while (per < 16 && 2 * per * per_token <= 768 && 2 * per * pairs <= kRopeSlots && A.tokens / (2 * per) >= 512) per *= 2;
     A.per_block = per;
     const int64_t blocks = (A.tokens + per - 1) / per;
     if (blocks > 0x7fffffffll) return COAT_ESHAPE;
     const dim3 grid((unsigned)blocks);
     hipStream_t st = (hipStream_t)stream;
-#define ROPE(DT)                                                                                  \
-    if (adjacent) hipLaunchKernelGGL((k_rope_axes<DT, true>), grid, dim3(256), 0, st, A);         \
-    else hipLaunchKernelGGL((k_rope_axes<DT, false>), grid, dim3(256), 0, st, A)
+#define ROPE(DT)                                                                                                    \
+    if (adjacent && whole) hipLaunchKernelGGL((k_rope_axes<DT, true, true>), grid, dim3(256), 0, st, A);             \
+    else if (adjacent) hipLaunchKernelGGL((k_rope_axes<DT, true, false>), grid, dim3(256), 0, st, A);                \
+    else if (whole) hipLaunchKernelGGL((k_rope_axes<DT, false, true>), grid, dim3(256), 0, st, A);                   \
+    else hipLaunchKernelGGL((k_rope_axes<DT, false, false>), grid, dim3(256), 0, st, A)
     if (dtype == COAT_F32) { ROPE(kF32); }
     else if (dtype == COAT_BF16) { ROPE(kBF16); }
     else { ROPE(kF16); }

@@ -294,7 +294,7 @@ int coat_rope_bf16(const void* x, void* y, const float* cos_tab, const float* si
  * turns by pos[axis[j]] * turns[j] whole turns: turns fp64 [pairs] = frequency / (2 pi), axis int32 [pairs] in [0, axes), both in
  * device memory.  adjacent 0: pair j is elements (j, j + pairs); 1: (2j, 2j + 1).  Elements from 2 * pairs on are copied.
  * inverse 1: the negated angle, which is the backward pass.  Angles are reduced in fp64, the rotation is fp32, rounded once.
- * Addresses need the element's own alignment only.  head_dim <= 2048, at most 4096 heads each. */
+ * Addresses need the element's own alignment only.  head_dim <= 2048, at most 1024 heads each. */
 int coat_rope_axes(const void* q, void* q_out, int64_t q_sb, int64_t q_ss, int64_t q_sh, int q_heads, const void* k, void* k_out,
                    int64_t k_sb, int64_t k_ss, int64_t k_sh, int k_heads, int dtype, const int64_t* pos, int64_t pos_sa,
                    int64_t pos_sb, int64_t pos_ss, int axes, const double* turns, const int32_t* axis, int pairs, int head_dim,
