@@ -8,6 +8,7 @@
 namespace coat {
 
 typedef uint32_t coat_u4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t coat_u2_at2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t coat_u4_at4 __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int DT> struct ElemBytes { static constexpr int value = DT == kF32 ? 4 : 2; };
@@ -118,6 +119,32 @@ template <int DT> __device__ __forceinline__ void store8(void* p, int64_t left, 
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++)
+            if (i < left) store_from_f32<DT>(p, i, v[i]);
+    }
+}
+// Four elements, for kernels whose widest tensors are fp32: lane l of a wave then reads bytes 16 l .. 16 l + 15 of one run with each
+// load (with eight fp32 elements a lane every load touches each line twice).
+template <int DT> __device__ __forceinline__ void load4(const void* p, int64_t left, float* o) {
+    if (left >= 4) {
+        if (DT == kF32) {
+            const coat_u4_at4 a = *(const coat_u4_at4*)p;
+            o[0] = u2f(a.x); o[1] = u2f(a.y); o[2] = u2f(a.z); o[3] = u2f(a.w);
+        } else {
+            const coat_u2_at2 a = *(const coat_u2_at2*)p;
+            o[0] = elem_lo<DT>(a.x); o[1] = elem_hi<DT>(a.x); o[2] = elem_lo<DT>(a.y); o[3] = elem_hi<DT>(a.y);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = i < left ? load_as_f32<DT>(p, i) : 0.0f;
+    }
+}
+template <int DT> __device__ __forceinline__ void store4(void* p, int64_t left, const float* v) {
+    if (left >= 4) {
+        if (DT == kF32) *(coat_u4_at4*)p = (coat_u4_at4){f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])};
+        else *(coat_u2_at2*)p = (coat_u2_at2){pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
             if (i < left) store_from_f32<DT>(p, i, v[i]);
     }
 }
