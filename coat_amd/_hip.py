@@ -74,6 +74,9 @@ SIGNATURES = {
     "coat_fp8_adamw_step": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _f, _i, _i, _i64, _i64, _vp],
     "coat_fp8_adamw_expand_step_multi": [_i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _f,
                                          _i, _i, _i, _vp],
+    "coat_fp8_adamw_expand_step_multi_scaled": [_i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _f,
+                                                _i, _i, _i, _vp, _vp],
+    "coat_fp8_adamw_step_multi_scaled": [_i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _f, _i, _i, _vp, _vp],
     "coat_layer_norm_forward": [_vp, _i64, _i, _vp, _vp, _i, _vp, _vp, _vp, _i64, _i64, _f, _vp],
     "coat_layer_norm_partials": [_i64, _i64],
     "coat_layer_norm_backward": [_vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i64, _i64, _vp],

@@ -32,6 +32,7 @@ struct AdamArgs {
     float one_minus_beta1, one_minus_beta2;
     float correction1, correction2_sqrt;  // 1 - beta1^step, sqrt(1 - beta2^step), evaluated on the host
     float expand_min;
+    const float* grad_scale;  // SCALED: one fp32 that the gradients are multiplied by
     float inv_expand_min;  // 1 / expand_min when expand_min is a power of two (the division is then a multiplication), else 0
 };
 
@@ -142,7 +143,7 @@ __device__ __forceinline__ void store_codes4(uint8_t* base, int64_t e, int64_t n
 // ------------------------------------------------------------------------------------------------
 // Plain (no expansion) step: every operation is the IEEE operation of the reference, bit-exact.
 // FULL: all eight groups of the wave are complete (no element or group masking anywhere).
-template <int PDT, bool FULL>
+template <int PDT, bool FULL, bool SCALED = false>
 __device__ __forceinline__ void adamw_plain_wave(void* __restrict__ params, const void* __restrict__ grads,
                                                  uint8_t* __restrict__ exp_avg, float* __restrict__ scale_m,
                                                  uint8_t* __restrict__ exp_avg_sq, float* __restrict__ scale_v,
@@ -164,7 +165,7 @@ __device__ __forceinline__ void adamw_plain_wave(void* __restrict__ params, cons
         cm[j] = load_codes4(exp_avg, e0 + 32 * j, numel);
         cv[j] = load_codes4(exp_avg_sq, e0 + 32 * j, numel);
     }
-    const float sm = scale_m[gidx], sv = scale_v[gidx];
+    const float sm = scale_m[gidx], sv = scale_v[gidx], gs = SCALED ? *A.grad_scale : 1.0f;
     float m[4][4], v[4][4];
     float mx_m = 0.0f, mx_v = 0.0f;
     uint32_t low_v = 0xFFFFFFFFu;  // smallest second moment other than +0, as bits - 1 (+0 wraps to the largest value)
@@ -177,7 +178,7 @@ __device__ __forceinline__ void adamw_plain_wave(void* __restrict__ params, cons
         for (int i = 0; i < 4; i++) {
             const bool ok = FULL || e0 + 32 * j + i < lim;
             float em = fm[i] * sm, ev = fv[i] * sv;
-            const float gr = g[j][i];
+            const float gr = SCALED ? g[j][i] * gs : g[j][i];
             em = A.beta1 * em + A.one_minus_beta1 * gr;
             ev = A.beta2 * ev + (A.one_minus_beta2 * gr) * gr;
             m[j][i] = em;
@@ -284,7 +285,7 @@ struct GroupIn {  // per-group constants of the incoming state
     float sm, sv, invk_m, invk_v, c_m, c_v;
 };
 
-template <int PDT, bool FULL>
+template <int PDT, bool FULL, bool SCALED = false>
 __device__ __forceinline__ void adamw_expand_wave(void* __restrict__ params, const void* __restrict__ grads,
                                                   uint8_t* __restrict__ exp_avg, float* __restrict__ scale_m,
                                                   float* __restrict__ expand_m, float* __restrict__ sqrtmm_m,
@@ -318,7 +319,7 @@ __device__ __forceinline__ void adamw_expand_wave(void* __restrict__ params, con
     // exponents outside (0, inf) need the special cases of powf; decided once per wave
     const bool odd_in = __builtin_amdgcn_ballot_w64(!(G.invk_m > 0.0f && G.invk_m < INFINITY) ||
                                                     !(G.invk_v > 0.0f && G.invk_v < INFINITY)) != 0;
-    const float inv_c2 = 1.0f / A.correction2_sqrt;
+    const float inv_c2 = 1.0f / A.correction2_sqrt, gs = SCALED ? *A.grad_scale : 1.0f;
 
     float m[4][4], v[4][4];
     float mx_m = 0.0f, mx_v = 0.0f, mn_m = kFltMax, mn_v = kFltMax;
@@ -340,7 +341,7 @@ __device__ __forceinline__ void adamw_expand_wave(void* __restrict__ params, con
                 em = copysignf(pow_full(fabsf(em), G.invk_m) * G.c_m, em);
                 ev = pow_full(ev, G.invk_v) * G.c_v;
             }
-            const float gr = g[j][i], pr = p[j][i];
+            const float gr = SCALED ? g[j][i] * gs : g[j][i], pr = p[j][i];
             em = fmaf(A.beta1, em, A.one_minus_beta1 * gr);
             ev = fmaf(A.beta2, ev, (A.one_minus_beta2 * gr) * gr);
             const float denom = fmaf(__builtin_amdgcn_sqrtf(ev), inv_c2, A.eps) * A.correction1;
@@ -490,7 +491,7 @@ struct AdamMultiArgs {
     int count;
 };
 
-template <int PDT, bool EXPAND>
+template <int PDT, bool EXPAND, bool SCALED>
 __global__ __launch_bounds__(256) void k_fp8_adamw_multi(AdamMultiArgs M, AdamArgs A) {
     enable_fp8_saturation();
     int ti = 0;  // the last tensor whose first block is not after this one (block-uniform, scalar registers)
@@ -504,16 +505,16 @@ __global__ __launch_bounds__(256) void k_fp8_adamw_multi(AdamMultiArgs M, AdamAr
     const bool full = (wave * 8 + 8) * kGroup <= numel;
     if (EXPAND) {
         if (full)
-            adamw_expand_wave<PDT, true>(T.params, T.grads, T.exp_avg, T.scale_m, T.expand_m, T.sqrtmm_m, T.exp_avg_sq, T.scale_v,
+            adamw_expand_wave<PDT, true, SCALED>(T.params, T.grads, T.exp_avg, T.scale_m, T.expand_m, T.sqrtmm_m, T.exp_avg_sq, T.scale_v,
                                          T.expand_v, T.sqrtmm_v, A, numel, ngroups, wave, lane);
         else
-            adamw_expand_wave<PDT, false>(T.params, T.grads, T.exp_avg, T.scale_m, T.expand_m, T.sqrtmm_m, T.exp_avg_sq, T.scale_v,
+            adamw_expand_wave<PDT, false, SCALED>(T.params, T.grads, T.exp_avg, T.scale_m, T.expand_m, T.sqrtmm_m, T.exp_avg_sq, T.scale_v,
                                           T.expand_v, T.sqrtmm_v, A, numel, ngroups, wave, lane);
     } else {
         if (full)
-            adamw_plain_wave<PDT, true>(T.params, T.grads, T.exp_avg, T.scale_m, T.exp_avg_sq, T.scale_v, A, numel, ngroups, wave, lane);
+            adamw_plain_wave<PDT, true, SCALED>(T.params, T.grads, T.exp_avg, T.scale_m, T.exp_avg_sq, T.scale_v, A, numel, ngroups, wave, lane);
         else
-            adamw_plain_wave<PDT, false>(T.params, T.grads, T.exp_avg, T.scale_m, T.exp_avg_sq, T.scale_v, A, numel, ngroups, wave, lane);
+            adamw_plain_wave<PDT, false, SCALED>(T.params, T.grads, T.exp_avg, T.scale_m, T.exp_avg_sq, T.scale_v, A, numel, ngroups, wave, lane);
     }
 }
 
@@ -530,6 +531,7 @@ static AdamArgs adam_args(float beta1, float beta2, float lr, float wd, float ep
     A.correction1 = 1.0f - (float)pow((double)beta1, (double)(float)step);
     A.correction2_sqrt = sqrtf(1.0f - (float)pow((double)beta2, (double)(float)step));
     A.expand_min = (float)expand_min;
+    A.grad_scale = nullptr;
     A.inv_expand_min = (expand_min > 0 && (expand_min & (expand_min - 1)) == 0) ? 1.0f / (float)expand_min : 0.0f;
     return A;
 }
@@ -594,7 +596,7 @@ static int adamw_multi(int count, void* const* params, const void* const* grads,
                        float* const* scale_m, float* const* expand_m, float* const* sqrtmm_m, void* const* exp_avg_sq,
                        float* const* scale_v, float* const* expand_v, float* const* sqrtmm_v, const int64_t* numel,
                        const int64_t* n_scale, float beta1, float beta2, float lr, float wd, float eps, int step,
-                       int qgroup_size, int expand_min, bool expand, void* stream) {
+                       int qgroup_size, int expand_min, bool expand, const float* grad_scale, void* stream) {
     if (qgroup_size != kGroup) return COAT_EQGROUP;
     if (count < 0) return COAT_EINVAL;
     if (count == 0) return COAT_OK;
@@ -610,7 +612,9 @@ static int adamw_multi(int count, void* const* params, const void* const* grads,
         if (!coat_aligned16(params[i]) || !coat_aligned16(grads[i]) || !coat_aligned16(exp_avg[i]) || !coat_aligned16(exp_avg_sq[i]))
             return COAT_EALIGN;
     }
-    const AdamArgs A = adam_args(beta1, beta2, lr, wd, eps, step, expand_min);
+    if ((uintptr_t)grad_scale & 3u) return COAT_EALIGN;
+    AdamArgs A = adam_args(beta1, beta2, lr, wd, eps, step, expand_min);
+    A.grad_scale = grad_scale;
     hipStream_t st = (hipStream_t)stream;
     AdamMultiArgs M;
     int i = 0;
@@ -636,15 +640,20 @@ static int adamw_multi(int count, void* const* params, const void* const* grads,
         }
         if (M.count == 0) break;  // only empty tensors were left
         M.first_block[M.count] = (unsigned)blocks;
-#define LAUNCH_MULTI(PDT)                                                                                             \
-    if (expand) hipLaunchKernelGGL((k_fp8_adamw_multi<PDT, true>), dim3((unsigned)blocks), dim3(256), 0, st, M, A);   \
-    else hipLaunchKernelGGL((k_fp8_adamw_multi<PDT, false>), dim3((unsigned)blocks), dim3(256), 0, st, M, A);
+#define LAUNCH_MULTI_AS(PDT, EXPAND, SCALED) \
+    hipLaunchKernelGGL((k_fp8_adamw_multi<PDT, EXPAND, SCALED>), dim3((unsigned)blocks), dim3(256), 0, st, M, A)
+#define LAUNCH_MULTI(PDT)                                                                   \
+    if (expand && grad_scale) LAUNCH_MULTI_AS(PDT, true, true);                             \
+    else if (expand) LAUNCH_MULTI_AS(PDT, true, false);                                     \
+    else if (grad_scale) LAUNCH_MULTI_AS(PDT, false, true);                                 \
+    else LAUNCH_MULTI_AS(PDT, false, false)
         switch (p_dtype) {
             case COAT_F32: LAUNCH_MULTI(kF32); break;
             case COAT_BF16: LAUNCH_MULTI(kBF16); break;
             default: LAUNCH_MULTI(kF16); break;
         }
 #undef LAUNCH_MULTI
+#undef LAUNCH_MULTI_AS
         const int rc = coat_launch_status();
         if (rc != COAT_OK) return rc;
     }
@@ -661,7 +670,7 @@ extern "C" int coat_fp8_adamw_expand_step_multi(int count, void* const* params, 
                                                 void* stream) {
     return adamw_multi(count, params, grads, p_dtype, exp_avg, scale_exp_avg, expand_exp_avg, sqrtminmax_exp_avg, exp_avg_sq,
                        scale_exp_avg_sq, expand_exp_avg_sq, sqrtminmax_exp_avg_sq, numel, n_scale, beta1, beta2, lr, wd, eps,
-                       step, qgroup_size, expand_min, true, stream);
+                       step, qgroup_size, expand_min, true, nullptr, stream);
 }
 
 extern "C" int coat_fp8_adamw_step_multi(int count, void* const* params, const void* const* grads, int p_dtype,
@@ -670,5 +679,27 @@ extern "C" int coat_fp8_adamw_step_multi(int count, void* const* params, const v
                                          float beta1, float beta2, float lr, float wd, float eps, int step, int qgroup_size,
                                          void* stream) {
     return adamw_multi(count, params, grads, p_dtype, exp_avg, scale_exp_avg, nullptr, nullptr, exp_avg_sq, scale_exp_avg_sq,
-                       nullptr, nullptr, numel, n_scale, beta1, beta2, lr, wd, eps, step, qgroup_size, 0, false, stream);
+                       nullptr, nullptr, numel, n_scale, beta1, beta2, lr, wd, eps, step, qgroup_size, 0, false, nullptr, stream);
+}
+
+extern "C" int coat_fp8_adamw_expand_step_multi_scaled(int count, void* const* params, const void* const* grads, int p_dtype,
+                                                       void* const* exp_avg, float* const* scale_exp_avg, float* const* expand_exp_avg,
+                                                       float* const* sqrtminmax_exp_avg, void* const* exp_avg_sq,
+                                                       float* const* scale_exp_avg_sq, float* const* expand_exp_avg_sq,
+                                                       float* const* sqrtminmax_exp_avg_sq, const int64_t* numel, const int64_t* n_scale,
+                                                       float beta1, float beta2, float lr, float wd, float eps, int step,
+                                                       int qgroup_size, int expand_min, const float* grad_scale, void* stream) {
+    if (!grad_scale) return COAT_EINVAL;
+    return adamw_multi(count, params, grads, p_dtype, exp_avg, scale_exp_avg, expand_exp_avg, sqrtminmax_exp_avg, exp_avg_sq,
+                       scale_exp_avg_sq, expand_exp_avg_sq, sqrtminmax_exp_avg_sq, numel, n_scale, beta1, beta2, lr, wd, eps, step,
+                       qgroup_size, expand_min, true, grad_scale, stream);
+}
+
+extern "C" int coat_fp8_adamw_step_multi_scaled(int count, void* const* params, const void* const* grads, int p_dtype, void* const* exp_avg,
+                                                float* const* scale_exp_avg, void* const* exp_avg_sq, float* const* scale_exp_avg_sq,
+                                                const int64_t* numel, const int64_t* n_scale, float beta1, float beta2, float lr, float wd,
+                                                float eps, int step, int qgroup_size, const float* grad_scale, void* stream) {
+    if (!grad_scale) return COAT_EINVAL;
+    return adamw_multi(count, params, grads, p_dtype, exp_avg, scale_exp_avg, nullptr, nullptr, exp_avg_sq, scale_exp_avg_sq, nullptr,
+                       nullptr, numel, n_scale, beta1, beta2, lr, wd, eps, step, qgroup_size, 0, false, grad_scale, stream);
 }

@@ -22,6 +22,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ._attention import sdpa
+from .rotary import RotaryAxes, rotary_axes
 from ..activation.real_quantization import (fp8_add_Ifp_Ifp_Ofp_Og16, fp8_add_Ifp_Ifp_Ofp_Opt, fp8_division,
                                             fp8_division_transpose, fp8_linear_backward, fp8_linear_backward_grouped,
                                             fp8_linear_forward, fp8_linear_forward_add, fp8_linear_forward_grouped,
@@ -509,6 +510,9 @@ class LlamaSdpaAttentionWithoutLinear(nn.Module):
         self.num_key_value_heads = config.num_key_value_heads
         self.num_key_value_groups = self.num_heads // self.num_key_value_heads
         self.rope_theta = config.rope_theta
+        # pairs of each position axis (time, height, width, ...), for position_ids of shape [axes, B, S]
+        sections = getattr(config, "rotary_sections", None)
+        self.rotary_axes = None if sections is None else RotaryAxes(self.head_dim, sections, theta=self.rope_theta)
         # formats in which the neighbouring FP8 modules quantize this module's output (forward) and the gradients of its
         # inputs (backward) per tensor: the kernels here hand them the scale maximum
         qargs = QuantizationConfig(**getattr(config, "coat_fp8_args", {}))
@@ -522,7 +526,18 @@ class LlamaSdpaAttentionWithoutLinear(nn.Module):
             raise NotImplementedError("KV caching is not part of the training path built here")
         bsz, q_len, _ = query_states.size()
         v = value_states.view(bsz, q_len, self.num_key_value_heads, self.head_dim).transpose(1, 2)
-        if position_embeddings is None and query_states.is_cuda and query_states.dtype == torch.bfloat16:
+        if position_embeddings is None and position_ids is not None and position_ids.dim() == 3:
+            if self.rotary_axes is None:
+                raise ValueError("position_ids with several axes need config.rotary_sections")
+            q = query_states.view(bsz, q_len, self.num_heads, self.head_dim)
+            k = key_states.view(bsz, q_len, self.num_key_value_heads, self.head_dim)
+            if q.is_cuda:
+                q, k = rotary_axes(q, k, position_ids, self.rotary_axes)
+                q, k = q.transpose(1, 2), k.transpose(1, 2)
+            else:  # evaluation on the CPU, in torch operations like the rest of the layer there
+                cos, sin = self.rotary_axes.cos_sin(position_ids, q.dtype)
+                q, k = apply_rotary_pos_emb(q.transpose(1, 2), k.transpose(1, 2), cos, sin)
+        elif position_embeddings is None and query_states.is_cuda and query_states.dtype == torch.bfloat16:
             # one fused kernel per tensor and direction instead of mul / neg / cat / add passes
             max_pos = getattr(self.config, "max_position_embeddings", None)
             grad_fp8 = self._grad_fp8 if self.training else None

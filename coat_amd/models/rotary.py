@@ -14,8 +14,8 @@ class RotaryAxes:
     ``sections``: pairs of each axis in turn; their sum P is the number of turning pairs, 2 P <= ``head_dim`` (the elements behind
     are passed through).  Pair j turns by ``position * theta ** -(j / P)``; with ``restart`` every section counts its own pairs,
     ``theta ** -(i / n)`` for pair i of a section of n.  Pair j is elements ``(j, j + P)`` of the head, the layout of the decoder
-    layers; with ``pairs`` neighbours ``(2 j, 2 j + 1)``.  The tables live on the device that is current at construction; another
-    device gets its own at the first use there (which must not be inside a graph capture)."""
+    layers; with ``pairs`` neighbours ``(2 j, 2 j + 1)``.  If CUDA is initialised, the tables are made on the device that is current
+    at construction; another device gets its own at the first use there (which must not be inside a graph capture)."""
 
     def __init__(self, head_dim, sections, theta=10000.0, restart=False, pairs=False):
         self.head_dim, self.sections, self.theta = int(head_dim), tuple(int(n) for n in sections), float(theta)
@@ -31,7 +31,7 @@ class RotaryAxes:
         exponent = [i / n for n in self.sections for i in range(n)] if self.restart else [j / total for j in range(total)]
         self._freq = [self.theta ** -e for e in exponent]  # radians a position, in 64 bits
         self._tables = {}
-        if torch.cuda.is_available():
+        if torch.cuda.is_initialized():
             self.tables(torch.device("cuda", torch.cuda.current_device()))
 
     def tables(self, device):
@@ -42,7 +42,10 @@ class RotaryAxes:
         return self._tables[device]
 
     def cos_sin(self, position_ids, dtype):
-        """cos / sin [B, S, 2 P] for the (j, j + P) layout, from torch operations on any device; position_ids [axes, B, S]."""
+        """cos / sin [B, S, head_dim] from torch operations on any device, for heads that turn whole in the (j, j + P) layout;
+        position_ids [axes, B, S]."""
+        if self.pairs or 2 * self.turning != self.head_dim:
+            raise ValueError("RotaryAxes.cos_sin: only for heads that turn whole, in the (j, j + P) layout")
         freq = torch.tensor(self._freq, dtype=torch.float64, device=position_ids.device)
         angle = position_ids[torch.tensor(self._axis, device=position_ids.device)].permute(1, 2, 0).double() * freq
         angle = torch.cat((angle, angle), -1)

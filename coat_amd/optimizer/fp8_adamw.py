@@ -42,7 +42,14 @@ class CoatAdamW(Optimizer):
         *,
         fused: Optional[bool] = None,
         multi_tensor: bool = True,
+        state_bits: int = 8,
+        master_weights: bool = False,
+        max_grad_norm: Optional[float] = None,
     ):
+        """``state_bits=32`` keeps both moments in fp32 (norm weights, embeddings); ``master_weights`` then also an fp32 copy of
+        16-bit parameters (state key ``master``).  Both may be given per parameter group.  ``max_grad_norm``: the gradients of
+        all groups are clipped to that global 2-norm inside the step (``grad_norm`` then holds the norm of the last step, on the
+        device; the gradients themselves stay as they are).  None of the three is in the reference."""
         # multi_tensor (not in the reference): parameters of one dtype, device and step count share kernel launches
         self.multi_tensor = multi_tensor
         self.qargs = QuantizationConfig() if qargs is None else qargs
@@ -64,7 +71,21 @@ class CoatAdamW(Optimizer):
             if getattr(self.qargs, name) != "E4M3":
                 raise ValueError(f"{name} must be E4M3: the optimizer kernels store both moments in e4m3")
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=amsgrad, fused=fused)
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError(f"Invalid max_grad_norm: {max_grad_norm}")
+        # only what differs from the reference's optimizer shows in the parameter groups
+        extra = dict(state_bits=(state_bits, 8), master_weights=(master_weights, False), max_grad_norm=(max_grad_norm, None))
+        defaults.update({k: v for k, (v, plain) in extra.items() if v != plain})
+        self.grad_norm = None
         super().__init__(params, defaults)
+
+    def add_param_group(self, param_group):
+        bits = param_group.get("state_bits", self.defaults.get("state_bits", 8))
+        if bits not in (8, 32):
+            raise ValueError(f"Invalid state_bits: {bits} (8 or 32)")
+        if param_group.get("master_weights", self.defaults.get("master_weights", False)) and bits != 32:
+            raise ValueError("master_weights needs state_bits=32")
+        super().add_param_group(param_group)
 
     # ------------------------------------------------------------------ state
     @property
@@ -93,6 +114,13 @@ class CoatAdamW(Optimizer):
             if expand:
                 state["expand_" + name] = torch.ones(ngroups, device=p.device, dtype=torch.float32)
                 state["sqrt_minmax_" + name] = torch.ones(ngroups, device=p.device, dtype=torch.float32)
+        return state
+
+    def _init_state32(self, p):
+        state = self.state[p]
+        state["step"] = torch.tensor(0.0)
+        for name in ("exp_avg", "exp_avg_sq"):
+            state[name] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
         return state
 
     @torch._disable_dynamo
@@ -146,6 +174,13 @@ class CoatAdamW(Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        max_grad_norm, scale = self.defaults.get("max_grad_norm"), None
+        if max_grad_norm is not None:
+            grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+            if any(g.is_sparse for g in grads):
+                raise RuntimeError("AdamW does not support sparse gradients")
+            if grads:
+                self.grad_norm, scale = qoptim_cuda.grad_norm_multi(grads, max_grad_norm)
         expand = self.use_expansion
         qgroup_size, expand_min = self.qargs.qgroup_size, self.qargs.expand_min
         for group in self.param_groups:
@@ -156,6 +191,7 @@ class CoatAdamW(Optimizer):
             # parameters of one dtype, device and step count are stepped together, 32 to a launch (the reference launches
             # once per parameter, :419-515); a parameter alone in its bucket takes the single-tensor entry point
             buckets = {}
+            bits, masters = group.get("state_bits", 8), group.get("master_weights", False)
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -163,15 +199,23 @@ class CoatAdamW(Optimizer):
                     raise RuntimeError("AdamW does not support sparse gradients")
                 state = self.state[p]
                 if len(state) == 0:
-                    state = self._init_state(p, expand)
+                    state = self._init_state(p, expand) if bits == 8 else self._init_state32(p)
                 state["step"] += 1
                 step = int(state["step"].item())
                 grad = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
                 if not p.is_contiguous():
                     raise RuntimeError("CoatAdamW needs contiguous parameters (the state is laid out flat)")
+                if masters and p.dtype != torch.float32 and "master" not in state:
+                    state["master"] = p.detach().float()
                 buckets.setdefault((p.dtype, p.device, step), []).append((p, grad, state))
-            for (_, _, step), items in buckets.items():
-                if len(items) == 1 or not getattr(self, "multi_tensor", True):
+            for (dtype, _, step), items in buckets.items():
+                if bits == 32:
+                    ps, gs, sts = map(list, zip(*items))
+                    copies = [st["master"] for st in sts] if masters and dtype != torch.float32 else None
+                    qoptim_cuda.adamw_step_multi(ps, gs, [st["exp_avg"] for st in sts], [st["exp_avg_sq"] for st in sts], beta1, beta2, lr,
+                                                 wd, eps, step, masters=copies, grad_scale=scale)
+                    continue
+                if scale is None and (len(items) == 1 or not getattr(self, "multi_tensor", True)):
                     for p, grad, state in items:
                         if expand:
                             qoptim_cuda.fp8_adamw_expand_step(
@@ -190,9 +234,9 @@ class CoatAdamW(Optimizer):
                     qoptim_cuda.fp8_adamw_expand_step_multi(
                         ps, gs, col("exp_avg"), col("scale_exp_avg"), col("expand_exp_avg"), col("sqrt_minmax_exp_avg"),
                         col("exp_avg_sq"), col("scale_exp_avg_sq"), col("expand_exp_avg_sq"), col("sqrt_minmax_exp_avg_sq"),
-                        beta1, beta2, lr, wd, eps, step, qgroup_size, expand_min)
+                        beta1, beta2, lr, wd, eps, step, qgroup_size, expand_min, grad_scale=scale)
                 else:
                     qoptim_cuda.fp8_adamw_step_multi(
                         ps, gs, col("exp_avg"), col("scale_exp_avg"), col("exp_avg_sq"), col("scale_exp_avg_sq"),
-                        beta1, beta2, lr, wd, eps, step, qgroup_size)
+                        beta1, beta2, lr, wd, eps, step, qgroup_size, grad_scale=scale)
         return loss

@@ -67,11 +67,16 @@ def fp8_adamw_step(params, grads, exp_avg, scale_exp_avg, exp_avg_sq, scale_exp_
         _hip.stream(params.device)), "fp8_adamw_step")
 
 
+def _check_grad_scale(what, grad_scale, index):
+    if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.get_device() != index:
+        raise RuntimeError(f"{what}: grad_scale must be one fp32 element on the parameters' device")
+
+
 def _pointer_array(tensors):
     return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
 
 
-def _multi(expand, params, grads, exp_avg, exp_avg_sq, scale_lists, hyper, step, qgroup_size, expand_min):
+def _multi(expand, params, grads, exp_avg, exp_avg_sq, scale_lists, hyper, step, qgroup_size, expand_min, grad_scale):
     n = len(params)
     if not (len(grads) == len(exp_avg) == len(exp_avg_sq) == n and all(len(l) == n for l in scale_lists)):
         raise RuntimeError("qoptim_cuda: the tensor lists differ in length")
@@ -84,6 +89,10 @@ def _multi(expand, params, grads, exp_avg, exp_avg_sq, scale_lists, hyper, step,
         ngroups.append(_common_checks(params[i], grads[i], exp_avg[i], exp_avg_sq[i], tuple(l[i] for l in scale_lists), qgroup_size))
         if any(l[i].numel() != ngroups[-1] for l in scale_lists):
             raise RuntimeError("grid_dim == scale_exp_avg_sq.numel()")
+    scaled, more = "", ()
+    if grad_scale is not None:
+        _check_grad_scale("qoptim_cuda", grad_scale, params[0].get_device())
+        scaled, more = "_scaled", (_hip.ptr(grad_scale),)
     numel = (ctypes.c_int64 * n)(*[t.numel() for t in params])
     n_scale = (ctypes.c_int64 * n)(*ngroups)
     arrays = [_pointer_array(l) for l in scale_lists]
@@ -91,32 +100,33 @@ def _multi(expand, params, grads, exp_avg, exp_avg_sq, scale_lists, hyper, step,
     lib, st = _hip.lib(), _hip.stream(params[0].device)
     if expand:
         sm, km, cm, sv, kv, cv = arrays
-        rc = lib.coat_fp8_adamw_expand_step_multi(n, _pointer_array(params), _pointer_array(grads), _hip.dt(params[0]),
-                                                  _pointer_array(exp_avg), sm, km, cm, _pointer_array(exp_avg_sq), sv, kv, cv,
-                                                  numel, n_scale, beta1, beta2, lr, wd, eps, int(step), int(qgroup_size),
-                                                  int(expand_min), st)
+        rc = getattr(lib, "coat_fp8_adamw_expand_step_multi" + scaled)(
+            n, _pointer_array(params), _pointer_array(grads), _hip.dt(params[0]), _pointer_array(exp_avg), sm, km, cm,
+            _pointer_array(exp_avg_sq), sv, kv, cv, numel, n_scale, beta1, beta2, lr, wd, eps, int(step), int(qgroup_size),
+            int(expand_min), *more, st)
     else:
         sm, sv = arrays
-        rc = lib.coat_fp8_adamw_step_multi(n, _pointer_array(params), _pointer_array(grads), _hip.dt(params[0]),
-                                           _pointer_array(exp_avg), sm, _pointer_array(exp_avg_sq), sv, numel, n_scale,
-                                           beta1, beta2, lr, wd, eps, int(step), int(qgroup_size), st)
+        rc = getattr(lib, "coat_fp8_adamw_step_multi" + scaled)(
+            n, _pointer_array(params), _pointer_array(grads), _hip.dt(params[0]), _pointer_array(exp_avg), sm,
+            _pointer_array(exp_avg_sq), sv, numel, n_scale, beta1, beta2, lr, wd, eps, int(step), int(qgroup_size), *more, st)
     _hip.check(rc, "fp8_adamw_expand_step_multi" if expand else "fp8_adamw_step_multi")
 
 
 def fp8_adamw_expand_step_multi(params, grads, exp_avg, scale_exp_avg, expand_exp_avg, sqrtminmax_exp_avg, exp_avg_sq,
                                 scale_exp_avg_sq, expand_exp_avg_sq, sqrtminmax_exp_avg_sq, beta1, beta2, lr, wd, eps, step,
-                                qgroup_size, expand_min):
-    """``fp8_adamw_expand_step`` on lists of tensors (one dtype, one device, one step count): one launch per 32 tensors."""
+                                qgroup_size, expand_min, grad_scale=None):
+    """``fp8_adamw_expand_step`` on lists of tensors (one dtype, one device, one step count): one launch per 32 tensors.
+    ``grad_scale``: a one-element fp32 tensor on the device that the gradients are multiplied by (``grad_norm_multi``)."""
     _multi(True, params, grads, exp_avg, exp_avg_sq,
            (scale_exp_avg, expand_exp_avg, sqrtminmax_exp_avg, scale_exp_avg_sq, expand_exp_avg_sq, sqrtminmax_exp_avg_sq),
-           (beta1, beta2, lr, wd, eps), step, qgroup_size, expand_min)
+           (beta1, beta2, lr, wd, eps), step, qgroup_size, expand_min, grad_scale)
 
 
 def fp8_adamw_step_multi(params, grads, exp_avg, scale_exp_avg, exp_avg_sq, scale_exp_avg_sq, beta1, beta2, lr, wd, eps,
-                         step, qgroup_size):
-    """``fp8_adamw_step`` on lists of tensors: one launch per 32 tensors."""
+                         step, qgroup_size, grad_scale=None):
+    """``fp8_adamw_step`` on lists of tensors: one launch per 32 tensors; ``grad_scale`` as above."""
     _multi(False, params, grads, exp_avg, exp_avg_sq, (scale_exp_avg, scale_exp_avg_sq), (beta1, beta2, lr, wd, eps), step,
-           qgroup_size, 0)
+           qgroup_size, 0, grad_scale)
 
 
 # ------------------------------------------------------------------------------------------------ 32-bit states, clipping
@@ -204,8 +214,8 @@ def adamw_step_multi(params, grads, exp_avg, exp_avg_sq, beta1, beta2, lr, wd, e
             raise RuntimeError("adamw_step_multi: a tensor that is stepped is given twice")
     if not int(step) >= 1:
         raise ValueError(f"adamw_step_multi: invalid step {step}")
-    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.get_device() != index):
-        raise RuntimeError("adamw_step_multi: grad_scale must be one fp32 element on the parameters' device")
+    if grad_scale is not None:
+        _check_grad_scale("adamw_step_multi", grad_scale, index)
     arrays = [array("Q", a) for a in addresses]
     numel, hyper = array("q", numel), array("d", (beta1, beta2, lr, wd, eps))
     _hip.launch("coat_adamw_step_multi", index, n, _address(arrays[0]), _hip.dt(pdt), _address(arrays[1]), _hip.dt(gdt),

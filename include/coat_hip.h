@@ -49,7 +49,7 @@ enum coat_fp8 { COAT_E4M3 = 0, COAT_E5M2 = 1 }; /* torch.float8_e4m3fn / torch.f
  * argument became COAT_MAX_WORDS words; 3: coat_fp8_gemm_residual, coat_fp8_rmsnorm_backward_add and coat_attention_forward_bf16 added,
  * coat_hbm_probe removed; 4: coat_rope_bf16 and coat_attention_forward_bf16 take a maximum buffer, the multi-tensor optimizer
  * steps and coat_fp8_layernorm_backward_add added; 5: coat_fp8_quantize_perblock added;
- * 6: coat_layer_norm_*, coat_rope_axes, coat_grad_norm_* and coat_adamw_step_multi added).  A caller compiled against this header checks coat_abi_version() == COAT_ABI_VERSION when it
+ * 6: coat_layer_norm_*, coat_rope_axes, coat_grad_norm_*, coat_adamw_step_multi and the _scaled multi-tensor steps added).  A caller compiled against this header checks coat_abi_version() == COAT_ABI_VERSION when it
  * loads the library. */
 #define COAT_ABI_VERSION 6
 int coat_abi_version(void);
@@ -404,6 +404,20 @@ int coat_fp8_adamw_step_multi(int count, void* const* params, const void* const*
                               float* const* scale_exp_avg, void* const* exp_avg_sq, float* const* scale_exp_avg_sq,
                               const int64_t* numel, const int64_t* n_scale, float beta1, float beta2, float lr, float wd,
                               float eps, int step, int qgroup_size, void* stream);
+
+/* The two multi-tensor steps with every gradient multiplied, in fp32, by *grad_scale (one fp32 in device memory, not NULL): the
+ * factor of coat_grad_norm_multi, so that clipping needs no pass over the gradients of its own. */
+int coat_fp8_adamw_expand_step_multi_scaled(int count, void* const* params, const void* const* grads, int p_dtype,
+                                            void* const* exp_avg, float* const* scale_exp_avg, float* const* expand_exp_avg,
+                                            float* const* sqrtminmax_exp_avg, void* const* exp_avg_sq,
+                                            float* const* scale_exp_avg_sq, float* const* expand_exp_avg_sq,
+                                            float* const* sqrtminmax_exp_avg_sq, const int64_t* numel, const int64_t* n_scale,
+                                            float beta1, float beta2, float lr, float wd, float eps, int step, int qgroup_size,
+                                            int expand_min, const float* grad_scale, void* stream);
+int coat_fp8_adamw_step_multi_scaled(int count, void* const* params, const void* const* grads, int p_dtype, void* const* exp_avg,
+                                     float* const* scale_exp_avg, void* const* exp_avg_sq, float* const* scale_exp_avg_sq,
+                                     const int64_t* numel, const int64_t* n_scale, float beta1, float beta2, float lr, float wd,
+                                     float eps, int step, int qgroup_size, const float* grad_scale, void* stream);
 
 /* The 2-norm of `count` gradient tensors taken together, and the factor that clips them to max_norm; no counterpart in the
  * reference.  grads, dtypes, numel: host arrays, read before the call returns (a tensor may be empty).  out: two fp32 in device

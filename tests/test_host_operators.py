@@ -187,3 +187,52 @@ def test_python_refusals_of_gpu_tensors(dev):
         with pytest.raises(RuntimeError, match="grad_scale"):
             step([a[0]], [a[1]], [a[2]], [a[3]], *hyper, grad_scale=bad)
     assert not any(t.any() for t in a)
+
+
+def test_scaled_fp8_step_entries(L, p):
+    i64, vp = ctypes.c_int64, ctypes.c_void_p
+    a, n, s, hp = (vp * 2)(p, p), (i64 * 2)(128, 256), (i64 * 2)(1, 2), (0.9, 0.95, 1e-3, 0.1, 1e-8, 1)
+    f, e = L.coat_fp8_adamw_step_multi_scaled, L.coat_fp8_adamw_expand_step_multi_scaled
+    assert f(2, a, a, 0, a, a, a, a, n, s, *hp, 128, None, None) == EINVAL  # a factor is what they are for
+    assert e(2, a, a, 0, a, a, a, a, a, a, a, a, n, s, *hp, 128, 16, None, None) == EINVAL
+    assert f(2, a, a, 0, a, a, a, a, n, s, *hp, 128, p + 2, None) == EALIGN
+    assert f(2, a, a, 0, a, a, a, a, n, s, *hp, 64, p, None) == -4
+    assert f(2, a, a, 7, a, a, a, a, n, s, *hp, 128, p, None) == EDTYPE
+    assert f(0, None, None, 0, None, None, None, None, None, None, *hp, 128, p, None) == 0
+
+
+def test_optimizer_refusals():
+    from coat_amd.optimizer.fp8_adamw import CoatAdamW
+    w = torch.nn.Parameter(torch.zeros(4))
+    for bad in (dict(state_bits=16), dict(master_weights=True), dict(max_grad_norm=-1.0), dict(max_grad_norm=float("nan"))):
+        with pytest.raises(ValueError):
+            CoatAdamW([w], **bad)
+    for bad in (dict(state_bits=4), dict(master_weights=True)):
+        with pytest.raises(ValueError):
+            CoatAdamW([dict(params=[w], **bad)])
+    opt = CoatAdamW([w])  # the reference's groups are unchanged where nothing is asked for
+    assert set(opt.param_groups[0]) == {"params", "lr", "betas", "eps", "weight_decay", "amsgrad", "fused"}
+    assert CoatAdamW([w], state_bits=32, max_grad_norm=0.0).param_groups[0]["state_bits"] == 32
+    w.grad = torch.zeros(4)
+    for kw in (dict(state_bits=32), dict(max_grad_norm=1.0)):
+        with pytest.raises(RuntimeError, match="GPU"):
+            CoatAdamW([w], **kw).step()
+
+
+def test_attention_module_evaluates_several_axes_on_the_cpu():
+    from coat_amd.models.coat_llama import CoatLlamaConfig, LlamaSdpaAttentionWithoutLinear, apply_rotary_pos_emb
+    g = torch.Generator().manual_seed(0)
+    config = CoatLlamaConfig(hidden_size=64, num_attention_heads=2, rotary_sections=(4, 6, 6))
+    module = LlamaSdpaAttentionWithoutLinear(config).eval()
+    q, k, v = (torch.randn(1, 7, 64, generator=g) for _ in range(3))
+    pos = torch.randint(0, 50, (3, 1, 7), generator=g)
+    out = module(q, k, v, position_ids=pos)[0]
+    freq = 10000.0 ** -(torch.arange(16, dtype=torch.float64) / 16)
+    ang = torch.cat((pos[0, 0, :, None] * freq[:4], pos[1, 0, :, None] * freq[4:10], pos[2, 0, :, None] * freq[10:]), -1)
+    ang = torch.cat((ang, ang), -1)[None]
+    heads = [t.view(1, 7, 2, 32).transpose(1, 2).double() for t in (q, k, v)]
+    rq, rk = apply_rotary_pos_emb(heads[0], heads[1], ang.cos(), ang.sin())
+    s = (rq @ rk.transpose(2, 3) / 32 ** 0.5).masked_fill(torch.triu(torch.ones(7, 7, dtype=torch.bool), 1), float("-inf")).softmax(-1)
+    assert torch.allclose(out.double(), (s @ heads[2]).transpose(1, 2).reshape(1, 7, 64), rtol=0, atol=1e-5)
+    with pytest.raises(ValueError, match="rotary_sections"):
+        LlamaSdpaAttentionWithoutLinear(CoatLlamaConfig(hidden_size=64, num_attention_heads=2))(q, k, v, position_ids=pos)
