@@ -32,7 +32,6 @@ struct AdamArgs {
     float one_minus_beta1, one_minus_beta2;
     float correction1, correction2_sqrt;  // 1 - beta1^step, sqrt(1 - beta2^step), evaluated on the host
     float expand_min;
-    const float* grad_scale;  // SCALED: one fp32 that the gradients are multiplied by
     float inv_expand_min;  // 1 / expand_min when expand_min is a power of two (the division is then a multiplication), else 0
 };
 
@@ -143,11 +142,13 @@ __device__ __forceinline__ void store_codes4(uint8_t* base, int64_t e, int64_t n
 // ------------------------------------------------------------------------------------------------
 // Plain (no expansion) step: every operation is the IEEE operation of the reference, bit-exact.
 // FULL: all eight groups of the wave are complete (no element or group masking anywhere).
+// SCALED: the gradients are multiplied by gs first.
 template <int PDT, bool FULL, bool SCALED = false>
 __device__ __forceinline__ void adamw_plain_wave(void* __restrict__ params, const void* __restrict__ grads,
                                                  uint8_t* __restrict__ exp_avg, float* __restrict__ scale_m,
                                                  uint8_t* __restrict__ exp_avg_sq, float* __restrict__ scale_v,
-                                                 const AdamArgs& A, int64_t numel_in, int64_t ngroups, int64_t wave, int lane) {
+                                                 const AdamArgs& A, int64_t numel_in, int64_t ngroups, int64_t wave, int lane,
+                                                 float gs = 1.0f) {
     const int lam = lane & 7;
     const int64_t gi = wave * 8 + (lane >> 3);
     const bool gvalid = FULL || gi < ngroups;
@@ -165,7 +166,7 @@ __device__ __forceinline__ void adamw_plain_wave(void* __restrict__ params, cons
         cm[j] = load_codes4(exp_avg, e0 + 32 * j, numel);
         cv[j] = load_codes4(exp_avg_sq, e0 + 32 * j, numel);
     }
-    const float sm = scale_m[gidx], sv = scale_v[gidx], gs = SCALED ? *A.grad_scale : 1.0f;
+    const float sm = scale_m[gidx], sv = scale_v[gidx];
     float m[4][4], v[4][4];
     float mx_m = 0.0f, mx_v = 0.0f;
     uint32_t low_v = 0xFFFFFFFFu;  // smallest second moment other than +0, as bits - 1 (+0 wraps to the largest value)
@@ -292,7 +293,7 @@ __device__ __forceinline__ void adamw_expand_wave(void* __restrict__ params, con
                                                   uint8_t* __restrict__ exp_avg_sq, float* __restrict__ scale_v,
                                                   float* __restrict__ expand_v, float* __restrict__ sqrtmm_v,
                                                   const AdamArgs& A, int64_t numel, int64_t ngroups, int64_t wave,
-                                                  int lane) {
+                                                  int lane, float gs = 1.0f) {
     const int lam = lane & 7;
     const int64_t gi = wave * 8 + (lane >> 3);
     const bool gvalid = FULL || gi < ngroups;
@@ -319,7 +320,7 @@ __device__ __forceinline__ void adamw_expand_wave(void* __restrict__ params, con
     // exponents outside (0, inf) need the special cases of powf; decided once per wave
     const bool odd_in = __builtin_amdgcn_ballot_w64(!(G.invk_m > 0.0f && G.invk_m < INFINITY) ||
                                                     !(G.invk_v > 0.0f && G.invk_v < INFINITY)) != 0;
-    const float inv_c2 = 1.0f / A.correction2_sqrt, gs = SCALED ? *A.grad_scale : 1.0f;
+    const float inv_c2 = 1.0f / A.correction2_sqrt;
 
     float m[4][4], v[4][4];
     float mx_m = 0.0f, mx_v = 0.0f, mn_m = kFltMax, mn_v = kFltMax;
@@ -492,8 +493,9 @@ struct AdamMultiArgs {
 };
 
 template <int PDT, bool EXPAND, bool SCALED>
-__global__ __launch_bounds__(256) void k_fp8_adamw_multi(AdamMultiArgs M, AdamArgs A) {
+__global__ __launch_bounds__(256) void k_fp8_adamw_multi(AdamMultiArgs M, AdamArgs A, const float* __restrict__ grad_scale) {
     enable_fp8_saturation();
+    const float gs = SCALED ? *grad_scale : 1.0f;
     int ti = 0;  // the last tensor whose first block is not after this one (block-uniform, scalar registers)
     for (int i = 1; i < M.count; i++)
         if (blockIdx.x >= M.first_block[i]) ti = i;
@@ -506,15 +508,15 @@ __global__ __launch_bounds__(256) void k_fp8_adamw_multi(AdamMultiArgs M, AdamAr
     if (EXPAND) {
         if (full)
             adamw_expand_wave<PDT, true, SCALED>(T.params, T.grads, T.exp_avg, T.scale_m, T.expand_m, T.sqrtmm_m, T.exp_avg_sq, T.scale_v,
-                                         T.expand_v, T.sqrtmm_v, A, numel, ngroups, wave, lane);
+                                         T.expand_v, T.sqrtmm_v, A, numel, ngroups, wave, lane, gs);
         else
             adamw_expand_wave<PDT, false, SCALED>(T.params, T.grads, T.exp_avg, T.scale_m, T.expand_m, T.sqrtmm_m, T.exp_avg_sq, T.scale_v,
-                                          T.expand_v, T.sqrtmm_v, A, numel, ngroups, wave, lane);
+                                          T.expand_v, T.sqrtmm_v, A, numel, ngroups, wave, lane, gs);
     } else {
         if (full)
-            adamw_plain_wave<PDT, true, SCALED>(T.params, T.grads, T.exp_avg, T.scale_m, T.exp_avg_sq, T.scale_v, A, numel, ngroups, wave, lane);
+            adamw_plain_wave<PDT, true, SCALED>(T.params, T.grads, T.exp_avg, T.scale_m, T.exp_avg_sq, T.scale_v, A, numel, ngroups, wave, lane, gs);
         else
-            adamw_plain_wave<PDT, false, SCALED>(T.params, T.grads, T.exp_avg, T.scale_m, T.exp_avg_sq, T.scale_v, A, numel, ngroups, wave, lane);
+            adamw_plain_wave<PDT, false, SCALED>(T.params, T.grads, T.exp_avg, T.scale_m, T.exp_avg_sq, T.scale_v, A, numel, ngroups, wave, lane, gs);
     }
 }
 
@@ -531,7 +533,6 @@ static AdamArgs adam_args(float beta1, float beta2, float lr, float wd, float ep
     A.correction1 = 1.0f - (float)pow((double)beta1, (double)(float)step);
     A.correction2_sqrt = sqrtf(1.0f - (float)pow((double)beta2, (double)(float)step));
     A.expand_min = (float)expand_min;
-    A.grad_scale = nullptr;
     A.inv_expand_min = (expand_min > 0 && (expand_min & (expand_min - 1)) == 0) ? 1.0f / (float)expand_min : 0.0f;
     return A;
 }
@@ -613,8 +614,7 @@ static int adamw_multi(int count, void* const* params, const void* const* grads,
             return COAT_EALIGN;
     }
     if ((uintptr_t)grad_scale & 3u) return COAT_EALIGN;
-    AdamArgs A = adam_args(beta1, beta2, lr, wd, eps, step, expand_min);
-    A.grad_scale = grad_scale;
+    const AdamArgs A = adam_args(beta1, beta2, lr, wd, eps, step, expand_min);
     hipStream_t st = (hipStream_t)stream;
     AdamMultiArgs M;
     int i = 0;
@@ -641,7 +641,7 @@ static int adamw_multi(int count, void* const* params, const void* const* grads,
         if (M.count == 0) break;  // only empty tensors were left
         M.first_block[M.count] = (unsigned)blocks;
 #define LAUNCH_MULTI_AS(PDT, EXPAND, SCALED) \
-    hipLaunchKernelGGL((k_fp8_adamw_multi<PDT, EXPAND, SCALED>), dim3((unsigned)blocks), dim3(256), 0, st, M, A)
+    hipLaunchKernelGGL((k_fp8_adamw_multi<PDT, EXPAND, SCALED>), dim3((unsigned)blocks), dim3(256), 0, st, M, A, grad_scale)
 #define LAUNCH_MULTI(PDT)                                                                   \
     if (expand && grad_scale) LAUNCH_MULTI_AS(PDT, true, true);                             \
     else if (expand) LAUNCH_MULTI_AS(PDT, true, false);                                     \

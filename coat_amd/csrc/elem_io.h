@@ -25,15 +25,17 @@ template <int DT> __device__ __forceinline__ uint32_t pack2(float lo, float hi) 
 template <int DT> struct Raw8 { uint32_t w[DT == kF32 ? 8 : 4]; };
 
 // p: address of the first element; left: elements from there to the end of the row (<= 0: nothing is read, zeros).
-template <int DT> __device__ __forceinline__ Raw8<DT> load_raw8(const void* p, int64_t left) {
+// STREAM: non-temporal loads, for a tensor that no later kernel reads again soon.
+template <int DT, bool STREAM = false> __device__ __forceinline__ Raw8<DT> load_raw8(const void* p, int64_t left) {
     Raw8<DT> r;
     if (left >= 8) {
         if (DT == kF32) {
-            const coat_u4_at4 a = ((const coat_u4_at4*)p)[0], b = ((const coat_u4_at4*)p)[1];
+            const coat_u4_at4* q = (const coat_u4_at4*)p;
+            const coat_u4_at4 a = STREAM ? __builtin_nontemporal_load(q) : q[0], b = STREAM ? __builtin_nontemporal_load(q + 1) : q[1];
             r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
             r.w[DT == kF32 ? 4 : 0] = b.x; r.w[DT == kF32 ? 5 : 1] = b.y; r.w[DT == kF32 ? 6 : 2] = b.z; r.w[DT == kF32 ? 7 : 3] = b.w;
         } else {
-            const coat_u4_at2 a = *(const coat_u4_at2*)p;
+            const coat_u4_at2 a = STREAM ? __builtin_nontemporal_load((const coat_u4_at2*)p) : *(const coat_u4_at2*)p;
             r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
         }
     } else if (left > 0) {  // all loads in flight together: elements past the end are read from the last one and cleared
@@ -56,13 +58,13 @@ template <int DT> __device__ __forceinline__ Raw8<DT> load_raw8(const void* p, i
 // The same for a load that is issued well before its use: the last piece of a row is read as the eight elements that end the row,
 // and settle_row8 moves them to their places when they are used.  (Picking single elements needs their values, that is a wait
 // right after the load: one lane of a block then holds up every row, 1.8x the time at 4100 columns.)
-template <int DT> __device__ __forceinline__ Raw8<DT> load_row8(const void* row, int c, int n, bool valid) {
+template <int DT, bool STREAM> __device__ __forceinline__ Raw8<DT> load_row8(const void* row, int c, int n, bool valid) {
     Raw8<DT> r;
 #pragma unroll
     for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = 0;
     if (valid && c < n) {
         if (n >= 8) {
-            r = load_raw8<DT>(elem_at<DT>(row, c + 8 <= n ? c : n - 8), 8);
+            r = load_raw8<DT, STREAM>(elem_at<DT>(row, c + 8 <= n ? c : n - 8), 8);
         } else {
             r = load_raw8<DT>(elem_at<DT>(row, c), n - c);
         }
@@ -70,12 +72,12 @@ template <int DT> __device__ __forceinline__ Raw8<DT> load_row8(const void* row,
     return r;
 }
 // RAGGED: n need not be a multiple of 8.  Otherwise c is below n only where a whole piece is.
-template <int DT, bool RAGGED> __device__ __forceinline__ Raw8<DT> load_piece(const void* row, int c, int n, bool valid = true) {
-    if (RAGGED) return load_row8<DT>(row, c, n, valid);
+template <int DT, bool RAGGED, bool STREAM> __device__ __forceinline__ Raw8<DT> load_piece(const void* row, int c, int n, bool valid = true) {
+    if (RAGGED) return load_row8<DT, STREAM>(row, c, n, valid);
     Raw8<DT> r;
 #pragma unroll
     for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = 0;
-    if (valid && c < n) r = load_raw8<DT>(elem_at<DT>(row, c), 8);
+    if (valid && c < n) r = load_raw8<DT, STREAM>(elem_at<DT>(row, c), 8);
     return r;
 }
 template <int DT> __device__ __forceinline__ void settle_row8(Raw8<DT>& r, int c, int n) {

@@ -68,7 +68,7 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __res
     Raw8<DT> raw[C];
     float wv[C][8], bv[C][8];
 #pragma unroll
-    for (int k = 0; k < C; k++) raw[k] = load_piece<DT, RAGGED>(elem_at<DT>(x, row * x_pitch), (k * lanes + l) * 8, N, row < M);
+    for (int k = 0; k < C; k++) raw[k] = load_piece<DT, RAGGED, false>(elem_at<DT>(x, row * x_pitch), (k * lanes + l) * 8, N, row < M);
 #pragma unroll
     for (int k = 0; k < C; k++) {
 #pragma unroll
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __res
             const int64_t next = row + step;
 #pragma unroll
             for (int k = 0; k < C; k++)
-                raw[k] = load_piece<DT, RAGGED>(elem_at<DT>(x, next * x_pitch), (k * lanes + l) * 8, N, next < M);
+                raw[k] = load_piece<DT, RAGGED, false>(elem_at<DT>(x, next * x_pitch), (k * lanes + l) * 8, N, next < M);
         }
         const float mean = row_sum<L>(s, red[0]) * inv_n;
         s = 0.0f;
@@ -123,6 +123,8 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __res
     }
 }
 
+// x and dy are not needed again after this kernel: streaming loads ([262144, 128] bf16: 42 -> 39 us with the sums; no difference at
+// 4096 columns; in the forward, whose x the backward reads, 24 -> 26).
 // dx, and with SUMS one partial row of dw and db per block (pw / pb may be NULL).
 template <int DT, int L, int C, bool RAGGED, bool SUMS>
 __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __restrict__ dy, int64_t dy_pitch, const void* __restrict__ x,
@@ -152,8 +154,8 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
 #pragma unroll
         for (int k = 0; k < C; k++) {
             const int c = (k * lanes + l) * 8;
-            rx[k] = load_piece<DT, RAGGED>(elem_at<DT>(x, at * x_pitch), c, N, at < M);
-            rg[k] = load_piece<DT, RAGGED>(elem_at<DT>(dy, at * dy_pitch), c, N, at < M);
+            rx[k] = load_piece<DT, RAGGED, true>(elem_at<DT>(x, at * x_pitch), c, N, at < M);
+            rg[k] = load_piece<DT, RAGGED, true>(elem_at<DT>(dy, at * dy_pitch), c, N, at < M);
         }
         mean = at < M ? mean_in[at] : 0.0f;
         rstd = at < M ? rstd_in[at] : 0.0f;

@@ -73,8 +73,8 @@ __global__ __launch_bounds__(256) void k_rope_axes(RopeArgs A) {
         const bool rest = J.piece >= turning;
         J.e = (rest ? J.piece - turning : J.piece) * 8;
         J.n = rest ? A.head_dim - rot : ADJ ? rot : A.pairs;
-        J.a = load_piece<DT, !WHOLE>(rest ? elem_at<DT>(x, rot) : x, J.e, J.n);
-        if (!ADJ && !rest) J.b = load_piece<DT, !WHOLE>(elem_at<DT>(x, A.pairs), J.e, J.n);
+        J.a = load_piece<DT, !WHOLE, true>(rest ? elem_at<DT>(x, rot) : x, J.e, J.n);
+        if (!ADJ && !rest) J.b = load_piece<DT, !WHOLE, true>(elem_at<DT>(x, A.pairs), J.e, J.n);
         return J;
     };
     Job J;

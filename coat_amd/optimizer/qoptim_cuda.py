@@ -130,6 +130,9 @@ def fp8_adamw_step_multi(params, grads, exp_avg, scale_exp_avg, exp_avg_sq, scal
 
 
 # ------------------------------------------------------------------------------------------------ 32-bit states, clipping
+_dtype_of = torch.Tensor.dtype.__get__  # without a Python frame per tensor
+
+
 def _columns(what, lists):
     """Checks parallel lists of tensors (name, tensors, dtype of all or None) that a multi-tensor call reads or writes flat: one
     length, one device, equal sizes, contiguous.  Returns (device index, sizes, addresses of each list)."""
@@ -143,7 +146,7 @@ def _columns(what, lists):
             raise RuntimeError(f"{what}: the tensor lists differ in length")
         if set(map(T.get_device, tensors)) != {index}:
             raise RuntimeError(f"{what}: {name} holds tensors that are not on the first tensor's device")
-        if dtype is not None and {t.dtype for t in tensors} != {dtype}:
+        if dtype is not None and set(map(_dtype_of, tensors)) != {dtype}:
             raise RuntimeError(f"{what}: {name} must all be {dtype}")
         if tensors is not first and list(map(T.numel, tensors)) != numel:
             raise RuntimeError(f"{what}: sizes of {name} differ from those of {lists[0][0]}")
@@ -173,7 +176,7 @@ def grad_norm_multi(grads, max_norm=None):
         grads = [g.contiguous() for g in grads]
     n = len(grads)
     index, numel, (addresses,) = _columns("grad_norm_multi", [("grads", grads, None)])
-    kinds = {g.dtype for g in grads}
+    kinds = set(map(_dtype_of, grads))
     dtypes = array("i", [_hip.dt(k) for k in kinds] * n if len(kinds) == 1 else [_hip.dt(g) for g in grads])
     numel, addresses = array("q", numel), array("Q", addresses)
     parts = _hip.lib().coat_grad_norm_partials(n, _address(numel))
