@@ -14,7 +14,8 @@ extern "C" const char* coat_status_string(int status) {
         case COAT_ESHAPE: return "shape contract violated (group / tile divisibility or scale length)";
         case COAT_EDTYPE: return "unsupported dtype combination";
         case COAT_EQGROUP: return "Only Support 128 per-group quantization currently";
-        case COAT_EALIGN: return "tensor base address must be 16-byte aligned";
+        case COAT_EALIGN: return "tensor base address is not aligned (16 bytes, or the element's size where the entry point asks for no more)";
+        case COAT_EOVERLAP: return "a tensor that is written shares memory with another tensor of the launch";
         default: return status > 0 ? hipGetErrorString((hipError_t)status) : "unknown coat status";
     }
 }

@@ -12,13 +12,15 @@
 // launch, nothing that a captured graph would have to keep alive.
 #include <math.h>
 
+#include <algorithm>
+
 #include "coat_host.h"
 #include "elem_io.h"
 
 namespace coat {
 
 // ------------------------------------------------------------------------------------------------ sum of squares
-constexpr int kNormMax = 128;        // tensors per launch
+constexpr int kNormMax = 184;        // tensors per launch: what the 4 KB of kernel arguments hold
 constexpr int kNormChunk = 8192;     // elements a block takes at a time
 constexpr int kNormBlocks = 2048;    // blocks (partial sums) per launch at most
 struct NormArgs {
@@ -116,7 +118,7 @@ __global__ __launch_bounds__(1024) void k_grad_norm(const double* __restrict__ p
 }
 
 // ------------------------------------------------------------------------------------------------ the step
-constexpr int kStepMax = 64;        // tensors per launch
+constexpr int kStepMax = 76;        // tensors per launch: what the 4 KB of kernel arguments hold
 constexpr int kStepChunk = 1024;    // elements a block steps
 struct Step32Tensor {
     void* p;
@@ -133,6 +135,8 @@ struct Step32Args {
 struct Hyper32 {
     float beta1, one_minus_beta1, beta2, one_minus_beta2, lr, wd, eps, c1, inv_c2;
 };
+
+static_assert(sizeof(NormArgs) + sizeof(double*) <= 4096 && sizeof(Step32Args) + sizeof(Hyper32) <= 4096, "kernel arguments");
 
 // One load of each stream a thread, and short blocks: the card holds enough of them to keep the memory busy (fp32, 333 M elements:
 // 1679 us or 5.56 TB/s; 2048 elements a block 1700, 4096 1736; non-temporal loads 1860).  The blocks go through the tensors from
@@ -196,6 +200,23 @@ template <typename F> static int for_each_launch(int count, const int64_t* numel
     return COAT_OK;
 }
 
+// Whether a tensor that is written shares memory with another tensor of a launch (a block would then read what another has
+// stepped already).  `spans`: begin, end and whether it is written; sorted here.
+struct Span {
+    uintptr_t begin, end;
+    bool written;
+};
+static bool overlap(Span* spans, int n) {
+    std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    uintptr_t end_any = 0, end_written = 0;
+    for (int i = 0; i < n; i++) {
+        if (spans[i].begin < (spans[i].written ? end_any : end_written)) return true;
+        if (spans[i].end > end_any) end_any = spans[i].end;
+        if (spans[i].written && spans[i].end > end_written) end_written = spans[i].end;
+    }
+    return false;
+}
+
 extern "C" int coat_grad_norm_partials(int count, const int64_t* numel) {
     if (count < 0 || (count > 0 && !numel)) return COAT_EINVAL;
     int64_t total = 0;
@@ -256,12 +277,29 @@ extern "C" int coat_adamw_step_multi(int count, void* const* params, int p_dtype
     if (!elem_aligned(grad_scale, COAT_F32)) return COAT_EALIGN;
     for (int i = 0; i < count; i++) {  // everything is checked before the first launch
         if (numel[i] < 0) return COAT_EINVAL;
+        if (numel[i] > ((int64_t)0x7fffffff) * kStepChunk) return COAT_ESHAPE;
         if (numel[i] == 0) continue;
         if (!params[i] || !grads[i] || !exp_avg[i] || !exp_avg_sq[i] || (masters && !masters[i])) return COAT_EINVAL;
         if (!elem_aligned(params[i], p_dtype) || !elem_aligned(grads[i], g_dtype) || !elem_aligned(exp_avg[i], COAT_F32) ||
             !elem_aligned(exp_avg_sq[i], COAT_F32) || (masters && !elem_aligned(masters[i], COAT_F32)))
             return COAT_EALIGN;
     }
+    const int checked = for_each_launch(count, numel, kStepChunk, kStepMax, [&](int first, int last, int64_t) {
+        Span spans[5 * kStepMax];
+        int n = 0;
+        for (int i = first; i < last; i++) {
+            const uintptr_t p = (uintptr_t)params[i], g = (uintptr_t)grads[i], m = (uintptr_t)exp_avg[i], v = (uintptr_t)exp_avg_sq[i];
+            const size_t size = (size_t)numel[i];
+            if (size == 0) continue;
+            spans[n++] = {p, p + size * (p_dtype == COAT_F32 ? 4 : 2), true};
+            spans[n++] = {g, g + size * (g_dtype == COAT_F32 ? 4 : 2), false};
+            spans[n++] = {m, m + size * 4, true};
+            spans[n++] = {v, v + size * 4, true};
+            if (masters) spans[n++] = {(uintptr_t)masters[i], (uintptr_t)masters[i] + size * 4, true};
+        }
+        return overlap(spans, n) ? COAT_EOVERLAP : COAT_OK;
+    });
+    if (checked != COAT_OK) return checked;
     // hyperparameters in double, rounded once: 1 - beta2 of a beta2 that was already rounded to fp32 is off by 1e-5 at 0.999
     const double beta1 = hyper[0], beta2 = hyper[1];
     Hyper32 H;

@@ -135,12 +135,13 @@ _dtype_of = torch.Tensor.dtype.__get__  # without a Python frame per tensor
 
 def _columns(what, lists):
     """Checks parallel lists of tensors (name, tensors, dtype of all or None) that a multi-tensor call reads or writes flat: one
-    length, one device, equal sizes, contiguous.  Returns (device index, sizes, addresses of each list)."""
+    length, one device, equal sizes, contiguous.  Returns (device index, sizes, addresses of each list), the latter two as host arrays
+    that an entry point can read."""
     first = lists[0][1]
     n, index, T = len(first), first[0].get_device(), torch.Tensor
     if index < 0:
         raise RuntimeError(f"{what}: tensors must be on the GPU")
-    numel, out = list(map(T.numel, first)), []
+    numel, out = array("q", map(T.numel, first)), []
     for name, tensors, dtype in lists:
         if len(tensors) != n:
             raise RuntimeError(f"{what}: the tensor lists differ in length")
@@ -148,11 +149,11 @@ def _columns(what, lists):
             raise RuntimeError(f"{what}: {name} holds tensors that are not on the first tensor's device")
         if dtype is not None and set(map(_dtype_of, tensors)) != {dtype}:
             raise RuntimeError(f"{what}: {name} must all be {dtype}")
-        if tensors is not first and list(map(T.numel, tensors)) != numel:
+        if tensors is not first and array("q", map(T.numel, tensors)) != numel:
             raise RuntimeError(f"{what}: sizes of {name} differ from those of {lists[0][0]}")
         if not all(map(T.is_contiguous, tensors)):
             raise RuntimeError(f"{what}: {name} must be contiguous")
-        out.append(list(map(T.data_ptr, tensors)))
+        out.append(array("Q", map(T.data_ptr, tensors)))
     return index, numel, out
 
 
@@ -178,7 +179,6 @@ def grad_norm_multi(grads, max_norm=None):
     index, numel, (addresses,) = _columns("grad_norm_multi", [("grads", grads, None)])
     kinds = set(map(_dtype_of, grads))
     dtypes = array("i", [_hip.dt(k) for k in kinds] * n if len(kinds) == 1 else [_hip.dt(g) for g in grads])
-    numel, addresses = array("q", numel), array("Q", addresses)
     parts = _hip.lib().coat_grad_norm_partials(n, _address(numel))
     if parts < 0:
         _hip.check(parts, "grad_norm_multi")
@@ -192,10 +192,11 @@ def grad_norm_multi(grads, max_norm=None):
 
 
 def adamw_step_multi(params, grads, exp_avg, exp_avg_sq, beta1, beta2, lr, wd, eps, step, masters=None, grad_scale=None):
-    """AdamW on lists of tensors with both moments in fp32, in place: one launch per 64 tensors, the formula of
+    """AdamW on lists of tensors with both moments in fp32, in place: one launch per 76 tensors, the formula of
     ``fp8_adamw_step``.  ``params`` share a dtype, ``grads`` have theirs or fp32.  ``masters``: fp32 copies of 16-bit parameters;
     they are stepped, and the parameters receive their rounding.  ``grad_scale``: a one-element fp32 tensor on the device that the
-    gradients are multiplied by (``grad_norm_multi``).  ``step`` counts from 1 and is read on the host: a captured graph keeps it."""
+    gradients are multiplied by (``grad_norm_multi``).  ``step`` counts from 1 and is read on the host: a captured graph keeps it.
+    Tensors that are stepped may share no memory with each other or with the gradients (RuntimeError)."""
     n = len(params)
     if n == 0:
         return
@@ -209,21 +210,22 @@ def adamw_step_multi(params, grads, exp_avg, exp_avg_sq, beta1, beta2, lr, wd, e
         raise RuntimeError(f"adamw_step_multi: grads dtype {gdt} is neither the params' {pdt} nor torch.float32")
     if masters is not None and pdt == torch.float32:
         raise RuntimeError("adamw_step_multi: masters are for parameters of 16 bits")
-    written = addresses[0] + [a for column in addresses[2:] for a in column]
-    if len(set(written)) != len(written):  # empty tensors share the address 0
-        sizes = numel * (len(addresses) - 1)
-        written = [a for a, size in zip(written, sizes) if size]
-        if len(set(written)) != len(written):
-            raise RuntimeError("adamw_step_multi: a tensor that is stepped is given twice")
+    if n > 76:  # more than one launch: the library compares the tensors of each
+        written = addresses[0]
+        for column in addresses[2:]:
+            written = written + column
+        if len(set(written)) != len(written):  # empty tensors share the address 0
+            written = [a for a, size in zip(written, numel * (len(addresses) - 1)) if size]
+            if len(set(written)) != len(written):
+                raise RuntimeError("adamw_step_multi: a tensor that is stepped is given twice")
     if not int(step) >= 1:
         raise ValueError(f"adamw_step_multi: invalid step {step}")
     if grad_scale is not None:
         _check_grad_scale("adamw_step_multi", grad_scale, index)
-    arrays = [array("Q", a) for a in addresses]
-    numel, hyper = array("q", numel), array("d", (beta1, beta2, lr, wd, eps))
-    _hip.launch("coat_adamw_step_multi", index, n, _address(arrays[0]), _hip.dt(pdt), _address(arrays[1]), _hip.dt(gdt),
-                _address(arrays[2]), _address(arrays[3]), _address(arrays[4]) if masters is not None else None, _address(numel),
-                _address(hyper), int(step), None if grad_scale is None else grad_scale.data_ptr(), what="adamw_step_multi")
+    p, g, m, v, w = (*map(_address, addresses), None)[:5]
+    hyper = array("d", (beta1, beta2, lr, wd, eps))
+    _hip.launch("coat_adamw_step_multi", index, n, p, _hip.dt(pdt), g, _hip.dt(gdt), m, v, w, _address(numel), _address(hyper),
+                int(step), None if grad_scale is None else grad_scale.data_ptr(), what="adamw_step_multi")
     # written behind autograd's back: graphs that saved them must notice
     try:
         torch.autograd.graph.increment_version(params)

@@ -112,6 +112,15 @@ def test_adamw_step_entry(L, p):
     assert f(2, a, 0, a, 0, a, a, None, n, h, 1, p + 2, None) == EALIGN
     assert f(1, a, 0, a, 0, a, a, None, (i64 * 1)(1 << 62), h, 1, None, None) == ESHAPE
     assert f(2, none, 0, none, 0, none, none, None, (i64 * 2)(0, 0), h, 1, None, None) == 0
+    # memory shared by a tensor that is written: 10 fp32 elements (40 bytes) from each of these
+    n10, EOVERLAP = (i64 * 2)(10, 10), -6
+    cols = [(vp * 2)(p + 400 * k, p + 400 * k + 200) for k in range(5)]
+    assert f(2, a, 0, cols[1], 0, cols[2], cols[3], None, n10, h, 1, None, None) == EOVERLAP                            # a tensor twice
+    assert f(2, (vp * 2)(p, p + 36), 0, cols[1], 0, cols[2], cols[3], None, n10, h, 1, None, None) == EOVERLAP          # the last element
+    assert f(2, cols[0], 0, cols[0], 0, cols[2], cols[3], None, n10, h, 1, None, None) == EOVERLAP                      # params as grads
+    assert f(2, cols[0], 0, (vp * 2)(p + 400, p + 836), 0, cols[2], cols[3], None, n10, h, 1, None, None) == EOVERLAP   # a grad into exp_avg
+    assert f(2, cols[0], 1, cols[1], 1, cols[2], cols[3], cols[3], n10, h, 1, None, None) == EOVERLAP                   # a master as a moment
+    assert b"shares memory" in L.coat_status_string(EOVERLAP)
 
 
 def test_python_refusals():
@@ -176,6 +185,12 @@ def test_python_refusals_of_gpu_tensors(dev):
                  (a[:2], [a[2], a[3].cpu()], a[4:6], a[6:])):
         with pytest.raises(RuntimeError):
             step(*args, *hyper)
+    flat = torch.zeros(200, 5, 8, device=dev)
+    many = [[flat[i, k] for i in range(200)] for k in (0, 1, 2, 3)]
+    many[0][150] = many[0][3]  # the same parameter twice, in two launches
+    with pytest.raises(RuntimeError, match="twice"):
+        step(*many, *hyper)
+    assert not flat.any()
     two = torch.zeros(8, 2, device=dev)[:, 0]
     with pytest.raises(RuntimeError, match="contiguous"):
         step([two], [a[1]], [a[2]], [a[3]], *hyper)
