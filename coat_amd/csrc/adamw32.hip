@@ -274,6 +274,7 @@ extern "C" int coat_adamw_step_multi(int count, void* const* params, int p_dtype
     if (count == 0) return COAT_OK;
     if (!params || !grads || !exp_avg || !exp_avg_sq || !numel || !hyper || step < 1) return COAT_EINVAL;
     if (!opt_dtype(p_dtype) || (g_dtype != p_dtype && g_dtype != COAT_F32) || (masters && p_dtype == COAT_F32)) return COAT_EDTYPE;
+    if (!(hyper[0] >= 0.0 && hyper[0] < 1.0) || !(hyper[1] >= 0.0 && hyper[1] < 1.0)) return COAT_EINVAL;
     if (!elem_aligned(grad_scale, COAT_F32)) return COAT_EALIGN;
     for (int i = 0; i < count; i++) {  // everything is checked before the first launch
         if (numel[i] < 0) return COAT_EINVAL;

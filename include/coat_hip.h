@@ -308,12 +308,12 @@ int coat_rope_axes(const void* q, void* q_out, int64_t q_sb, int64_t q_ss, int64
  * element's own alignment only.  Sums are fp32, the variance is the two-pass one, y is rounded once. */
 int coat_layer_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const void* w, const void* b, int w_dtype, void* y,
                             float* mean, float* rstd, int64_t M, int64_t N, float eps, void* stream);
-/* Partial rows that coat_layer_norm_backward makes use of for such a tensor (the n_partial to allocate), or a negative status. */
+/* The n_partial with which coat_layer_norm_backward is fastest on such a tensor, or a negative status. */
 int coat_layer_norm_partials(int64_t M, int64_t N);
 /* dx (dense, x_dtype), dw and db (w_dtype), each optional (NULL).  dy, x of x_dtype with row pitches (0 = N).  partial: fp32
- * workspace [2, n_partial, N] if both dw and db are wanted, [1, n_partial, N] for one, unused for none; 1 <= n_partial <= 65535,
- * more than coat_layer_norm_partials(M, N) are not used.  The partial rows are summed in a fixed order: the same bits every time
- * for one n_partial.  M = 0 gives zero gradients. */
+ * workspace [2, n_partial, N] if both dw and db are wanted, [1, n_partial, N] for one, unused for none; 1 <= n_partial <= 65535
+ * blocks each sum their rows into one partial row, which are then added in a fixed order: the same bits every time for one
+ * n_partial.  M = 0 gives zero gradients. */
 int coat_layer_norm_backward(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, int x_dtype, const float* mean,
                              const float* rstd, const void* w, int w_dtype, void* dx, void* dw, void* db, float* partial,
                              int n_partial, int64_t M, int64_t N, void* stream);
@@ -431,7 +431,8 @@ int coat_grad_norm_multi(int count, const void* const* grads, const int* dtypes,
 
 /* AdamW step of several tensors with both moments in fp32, 76 tensors to a launch; the formula of coat_fp8_adamw_step_multi.
  * params of p_dtype; grads of p_dtype or fp32; masters NULL, or fp32 copies of 16-bit parameters that are stepped instead, the
- * parameter receiving their rounding.  hyper: host array of five doubles: beta1, beta2, lr, weight decay, eps.  grad_scale: NULL,
+ * parameter receiving their rounding.  hyper: host array of five doubles: beta1, beta2 (both in [0, 1)), lr, weight decay,
+ * eps.  grad_scale: NULL,
  * or one fp32 in device memory that the gradients are multiplied by (out[1] above).  Host arrays are read before the call
  * returns; addresses need the element's own alignment only; a tensor that is written may share no memory with another
  * tensor (COAT_EOVERLAP where two of one launch do); empty ones are skipped; everything is checked before the first launch. */

@@ -98,6 +98,8 @@ def test_adamw_step_entry(L, p):
     assert f(0, None, 0, None, 0, None, None, None, None, None, 1, None, None) == 0
     assert f(2, a, 0, a, 0, a, a, None, n, h, 0, None, None) == EINVAL        # steps count from 1
     assert f(2, a, 0, a, 0, a, a, None, n, None, 1, None, None) == EINVAL
+    for bad in ((1.0, 0.9), (0.9, 1.0), (-0.1, 0.9), (float("nan"), 0.9)):
+        assert f(2, a, 0, a, 0, a, a, None, n, (ctypes.c_double * 5)(*bad, 1e-3, 0.1, 1e-8), 1, None, None) == EINVAL
     assert f(2, a, 5, a, 5, a, a, None, n, h, 1, None, None) == EDTYPE
     assert f(2, a, 0, a, 1, a, a, None, n, h, 1, None, None) == EDTYPE        # bf16 gradients of fp32 parameters
     assert f(2, a, 1, a, 2, a, a, None, n, h, 1, None, None) == EDTYPE
