@@ -21,7 +21,7 @@ def _rows(t, N):
 
 
 def _dense_like(t):
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 def _check(who, x, weight, bias):
@@ -54,7 +54,7 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
         raise ValueError(f"layer_norm_forward: invalid eps {eps}")
     N = x.shape[-1]
     y = _dense_like(x)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     x, pitch = _rows(x, N)
     w = weight if weight is None else weight.contiguous()
@@ -86,7 +86,8 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, bias_grad=True, *, x_gra
         parts = _hip.lib().coat_layer_norm_partials(M, N)
         if parts < 0:
             _hip.check(parts, "layer_norm_backward")
-        partial = torch.empty((wanted, parts, N), dtype=torch.float32, device=device)
+        if parts > 1 or N > 16384:  # one block writes the sums themselves
+            partial = x.new_empty((wanted, parts, N), dtype=torch.float32)
     x, x_pitch = _rows(x, N)
     dy, dy_pitch = _rows(dy, N)
     _hip.launch("coat_layer_norm_backward", x.get_device(), dy.data_ptr(), dy_pitch, x.data_ptr(), x_pitch, _hip.dt(x), mean.data_ptr(),

@@ -157,4 +157,15 @@ __device__ __forceinline__ void load8_rt(const void* p, int dt, int64_t i, int64
     else load8<kF16>(elem_at<kF16>(p, i), n - i, o);
 }
 
+__device__ __forceinline__ void store8_rt(void* p, int dt, int64_t i, int64_t n, const float* v) {
+    if (dt == kF32) store8<kF32>(elem_at<kF32>(p, i), n - i, v);
+    else if (dt == kBF16) store8<kBF16>(elem_at<kBF16>(p, i), n - i, v);
+    else store8<kF16>(elem_at<kF16>(p, i), n - i, v);
+}
+__device__ __forceinline__ void store_rt(void* p, int dt, int64_t i, float v) {
+    if (dt == kF32) store_from_f32<kF32>(p, i, v);
+    else if (dt == kBF16) store_from_f32<kBF16>(p, i, v);
+    else store_from_f32<kF16>(p, i, v);
+}
+
 }  // namespace coat

@@ -125,13 +125,14 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __res
 
 // x and dy are not needed again after this kernel: streaming loads ([262144, 128] bf16: 42 -> 39 us with the sums; no difference at
 // 4096 columns; in the forward, whose x the backward reads, 24 -> 26).
-// dx, and with SUMS one partial row of dw and db per block (pw / pb may be NULL).
+// dx, and with SUMS the sums for dw and db (either may be NULL): one partial row per block, in pw / pb, or, if there is one block
+// only, dw and db themselves.
 template <int DT, int L, int C, bool RAGGED, bool SUMS>
 __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __restrict__ dy, int64_t dy_pitch, const void* __restrict__ x,
                                                                  int64_t x_pitch, const float* __restrict__ mean_in,
                                                                  const float* __restrict__ rstd_in, const void* __restrict__ w, int w_dt,
-                                                                 void* __restrict__ dx, float* __restrict__ pw, float* __restrict__ pb,
-                                                                 int64_t M, int N) {
+                                                                 void* __restrict__ dx, void* __restrict__ dw, void* __restrict__ db,
+                                                                 float* __restrict__ pw, float* __restrict__ pb, int64_t M, int N) {
     constexpr int R = form_rows(L);
     constexpr bool kShared = SUMS && R > 1;  // several rows of the block share a column: summed through LDS at the end
     constexpr bool kLean = C * (DT == kF32 ? 2 : 1) * (RAGGED ? 2 : 1) >= 8;  // no registers left for the next row
@@ -225,17 +226,24 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
         }
     }
     if (SUMS) {
+        const bool alone = gridDim.x == 1;
         if (!kShared) {
 #pragma unroll
             for (int k = 0; k < C; k++) {
                 const int c = (k * lanes + l) * 8;
-                if (pw) store8<kF32>(pw + blockIdx.x * (int64_t)N + c, N - c, aw[k]);
-                if (pb) store8<kF32>(pb + blockIdx.x * (int64_t)N + c, N - c, ab[k]);
+                if (alone) {
+                    if (dw) store8_rt(dw, w_dt, c, N, aw[k]);
+                    if (db) store8_rt(db, w_dt, c, N, ab[k]);
+                } else {
+                    if (dw) store8<kF32>(pw + blockIdx.x * (int64_t)N + c, N - c, aw[k]);
+                    if (db) store8<kF32>(pb + blockIdx.x * (int64_t)N + c, N - c, ab[k]);
+                }
             }
         } else {
 #pragma unroll
             for (int which = 0; which < 2; which++) {
-                float* out = which == 0 ? pw : pb;
+                void* out = which == 0 ? dw : db;
+                float* part = which == 0 ? pw : pb;
                 if (!out) continue;
                 __syncthreads();
 #pragma unroll
@@ -246,7 +254,8 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
                 for (int c = threadIdx.x; c < N; c += 256) {
                     float s = cols[0][kShared ? c : 0];
                     for (int k = 1; k < R; k++) s += cols[kShared ? k : 0][kShared ? c : 0];
-                    out[blockIdx.x * (int64_t)N + c] = s;
+                    if (alone) store_rt(out, w_dt, c, s);
+                    else part[blockIdx.x * (int64_t)N + c] = s;
                 }
             }
         }
@@ -393,9 +402,7 @@ __global__ __launch_bounds__(kSumCols* kSumSlices) void k_ln_sum_partials(const 
         s = red[0][col];
 #pragma unroll
         for (int k = 1; k < kSumSlices; k++) s += red[k][col];
-        if (dt == kF32) store_from_f32<kF32>(out, c, s);
-        else if (dt == kBF16) store_from_f32<kBF16>(out, c, s);
-        else store_from_f32<kF16>(out, c, s);
+        store_rt(out, dt, c, s);
     }
 }
 
@@ -482,6 +489,8 @@ extern "C" int coat_layer_norm_partials(int64_t M, int64_t N) {
     // 4096 bf16: 41 us with 256, 43 with 384, 49 with 1024).  With few rows, fewer: a partial row costs as much to write and to
     // sum as it saves (1024 x 4096 bf16: 14 us with 192, 23 with 1024; the factor is fitted to such sweeps).
     const int threads = ln_shape(N, true).threads ? ln_shape(N, true).threads : 256;
+    // A few rows take one block, which needs no second kernel ([4, 4096] bf16: 12 us a call instead of 18).
+    if (ln_shape(N, true).threads && ln_rounds(M, N) <= 8) return 1;
     const int64_t rounds = ln_rounds(M, N), per_cu = N > 8192 || threads > 960 ? 1 : 960 / threads > 4 ? 4 : 960 / threads, most = 256 * per_cu;
     const double balanced = sqrt(27.0 * (double)rounds * (N < 4096 ? 4096.0 / (double)N : 1.0));
     int64_t n = balanced < (double)most ? (int64_t)balanced : most;
@@ -500,13 +509,13 @@ static int ln_backward(const void* dy, int64_t dy_pitch, const void* x, int64_t 
 #define BACKWARD(SUMS, BLOCKS)                                                                                                           \
     ln_form<SUMS>(N, [&](auto lanes, auto pieces, auto ragged) {                                                                         \
         hipLaunchKernelGGL((k_ln_bwd<DT, decltype(lanes)::value, decltype(pieces)::value, decltype(ragged)::value, SUMS>), dim3(BLOCKS), \
-                           dim3(shape.threads), 0, st, dy, dy_pitch, x, x_pitch, mean, rstd, w, w_dtype, dx, dw ? pw : nullptr,          \
-                           db ? pb : nullptr, M, (int)N);                                                                                \
+                           dim3(shape.threads), 0, st, dy, dy_pitch, x, x_pitch, mean, rstd, w, w_dtype, dx, dw, db, pw, pb, M, (int)N);                                       \
     })
         if (sums) BACKWARD(true, (unsigned)n_partial);
         else BACKWARD(false, ln_blocks(M, N, shape.threads));
 #undef BACKWARD
         if (const int rc = coat_launch_status()) return rc;
+        if (sums && n_partial == 1) return COAT_OK;
     } else if (M > 0) {
         if (dx) {
             hipLaunchKernelGGL((k_ln_bwd_long<DT>), dim3((unsigned)(M < 65536 ? M : 65536)), dim3(256), 0, st, dy, dy_pitch, x, x_pitch, mean,
@@ -537,7 +546,8 @@ extern "C" int coat_layer_norm_backward(const void* dy, int64_t dy_pitch, const 
     if (x_pitch == 0) x_pitch = N;
     if (dy_pitch == 0) dy_pitch = N;
     if (x_pitch < N || dy_pitch < N) return COAT_ESHAPE;
-    if ((dw || db) && M > 0 && (!partial || n_partial < 1 || n_partial > 65535)) return COAT_EINVAL;
+    const bool one_block = n_partial == 1 && ln_shape(N, true).threads;  // writes the sums themselves
+    if ((dw || db) && M > 0 && ((!partial && !one_block) || n_partial < 1 || n_partial > 65535)) return COAT_EINVAL;
     if (M > 0 && (!dy || !x || !mean || !rstd)) return COAT_EINVAL;
     if (!ln_aligned(dy, x_dtype) || !ln_aligned(x, x_dtype) || !ln_aligned(dx, x_dtype) || !ln_aligned(mean, COAT_F32) ||
         !ln_aligned(rstd, COAT_F32) || !ln_aligned(partial, COAT_F32) || (w && !ln_aligned(w, w_dtype)) || (dw && !ln_aligned(dw, w_dtype)) ||

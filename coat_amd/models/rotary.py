@@ -89,7 +89,7 @@ def _rotate(q, k, position_ids, plan, inverse):
         if t.stride(3) != 1:
             t = t.contiguous()
         kept.append(t)
-        out = torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=device)
+        out = torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
         outs.append(out)
         args += (t.data_ptr(), out.data_ptr(), *t.stride()[:3], t.shape[2])
     _hip.launch("coat_rope_axes", first.get_device(), *args, _hip.dt(first), pos.data_ptr(), *pos.stride(), len(plan.sections),

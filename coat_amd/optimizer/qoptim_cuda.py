@@ -182,9 +182,8 @@ def grad_norm_multi(grads, max_norm=None):
     parts = _hip.lib().coat_grad_norm_partials(n, _address(numel))
     if parts < 0:
         _hip.check(parts, "grad_norm_multi")
-    device = grads[0].device
-    work = torch.empty(max(parts, 1), dtype=torch.float64, device=device)
-    out = torch.empty(2, dtype=torch.float32, device=device)
+    work = grads[0].new_empty(max(parts, 1), dtype=torch.float64)
+    out = grads[0].new_empty(2, dtype=torch.float32)
     _hip.launch("coat_grad_norm_multi", index, n, _address(addresses), _address(dtypes), _address(numel),
                 0.0 if max_norm is None else float(max_norm), work.data_ptr(), parts, out.data_ptr(), what="grad_norm_multi")
     norm, scale = out.unbind()
