@@ -89,6 +89,29 @@ SIGNATURES = {
 }
 
 _lib = None
+_native = None
+
+
+def native():
+    """The compiled binding (coat_amd/_binding.so) of the operators whose small calls are bound by the host, holding this library's
+    entry points; raises if it has not been built (python -m coat_amd.build)."""
+    global _native
+    if _native is None:
+        L = lib()
+        try:
+            from . import _binding
+        except ImportError as e:
+            raise RuntimeError("coat_amd: _binding.so is missing or was built for another torch; build it with `python -m coat_amd.build` "
+                               f"(there is no fallback path): {e}") from e
+        if _binding.ABI_VERSION != ABI_VERSION:
+            raise RuntimeError(f"coat_amd: _binding.so has ABI version {_binding.ABI_VERSION}, this package needs {ABI_VERSION}; rebuild it "
+                               "with `python -m coat_amd.build`")
+        names = ("coat_status_string", "coat_layer_norm_forward", "coat_layer_norm_partials", "coat_layer_norm_backward", "coat_rope_axes",
+                 "coat_grad_norm_partials", "coat_grad_norm_multi", "coat_adamw_step_multi")
+        stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+        _binding.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names}, stream_of)
+        _native = _binding
+    return _native
 
 
 def lib():
@@ -140,24 +163,6 @@ def fp8(dtype):
 
 def stream(device=None):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
-# the current stream's handle and the current device without the Python objects around them (2 us less a call)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-
-
-def launch(name, device, *args, what=None):
-    """Calls entry point ``name`` with ``args`` and the current stream of ``device`` (its index), with that device current for the
-    launch, and raises on a status other than 0.  Pointers are plain integers (``Tensor.data_ptr()``) or None."""
-    fn = getattr(_lib or lib(), name)
-    if device == _current_device():
-        status = fn(*args, _raw_stream(device))
-    else:
-        with torch.cuda.device(device):
-            status = fn(*args, _raw_stream(device))
-    if status:
-        check(status, what or name)
 
 
 def ptr(t):

@@ -1,6 +1,6 @@
 """Builds libcoat_hip.so (the C-ABI library of hand-written gfx950 kernels) in-tree with hipcc.
 
-    python -m coat_amd.build            # compile every csrc/*.hip and link coat_amd/libcoat_hip.so
+    python -m coat_amd.build            # compile every csrc/*.hip and link coat_amd/libcoat_hip.so; compile coat_amd/_binding.so
 
 Cross-compiles without a GPU.  Flags that matter for numerics:
   -ffp-contract=off                              no implicit FMA: kernels state every fused operation explicitly
@@ -8,14 +8,17 @@ Cross-compiles without a GPU.  Flags that matter for numerics:
 """
 import concurrent.futures
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "csrc", "_obj")
 LIB = os.path.join(HERE, "libcoat_hip.so")
+BINDING = os.path.join(HERE, "_binding.so")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
@@ -36,6 +39,22 @@ def _compile(src):
     return src, obj, r.returncode, r.stdout + r.stderr
 
 
+def build_binding(verbose=True):
+    """Host-side Python binding (csrc/binding.cpp) against torch's C++ headers: no device code."""
+    torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]
+    src = os.path.join(CSRC, "binding.cpp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden",
+           "-I" + os.path.join(torch_dir, "include"), "-I" + os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING, "-L" + os.path.join(torch_dir, "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src}:\n" + r.stdout + r.stderr)
+    if verbose:
+        print(f"[coat_amd.build] compiled {BINDING}")
+    return BINDING
+
+
 def build(verbose=True, jobs=None, lib=None):
     lib = lib or os.environ.get("COAT_LIB_OUT") or LIB
     os.makedirs(OBJ, exist_ok=True)
@@ -43,6 +62,7 @@ def build(verbose=True, jobs=None, lib=None):
     jobs = jobs or min(len(srcs), int(os.environ.get("MAX_JOBS", "8")))
     objs = []
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as ex:
+        binding = ex.submit(build_binding, verbose)
         for src, obj, rc, out in ex.map(_compile, srcs):
             # hipcc's host pass warns that it does not know the packed-fp32 feature: harmless
             msgs = [l for l in out.splitlines() if "packed-fp32-ops" not in l and "is not a recognized feature" not in l]
@@ -54,6 +74,7 @@ def build(verbose=True, jobs=None, lib=None):
                 for l in warn[:10]:
                     print("   ", l)
             objs.append(obj)
+        binding.result()
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", lib, *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

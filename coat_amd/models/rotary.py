@@ -1,5 +1,6 @@
 """Rotary positions with several axes (time, height, width of video, image and text tokens) on q and k together, beside the one-axis
-rotary of the decoder layers (``coat_llama.fused_rotary``).  Kernel: coat_amd/csrc/rope_axes.hip."""
+rotary of the decoder layers (``coat_llama.fused_rotary``).  Kernel: coat_amd/csrc/rope_axes.hip; arguments are checked and outputs
+allocated in coat_amd/csrc/binding.cpp."""
 import math
 
 import torch
@@ -52,49 +53,12 @@ class RotaryAxes:
         return angle.cos().to(dtype), angle.sin().to(dtype)
 
 
-def _positions(position_ids, plan, B, S, device):
-    if position_ids.dim() != 3 or position_ids.shape[0] != len(plan.sections):
-        raise ValueError(f"rotary_axes: expected position_ids of shape [{len(plan.sections)}, batch, seq], got {tuple(position_ids.shape)}")
-    if position_ids.device != device:
-        raise ValueError(f"rotary_axes: position_ids are on {position_ids.device}, q and k on {device}")
-    if position_ids.dtype != torch.int64:
-        if position_ids.dtype.is_floating_point or position_ids.dtype.is_complex or position_ids.dtype == torch.bool:
-            raise ValueError(f"rotary_axes: position_ids must be whole numbers, got {position_ids.dtype}")
-        position_ids = position_ids.long()
-    return position_ids if position_ids.shape[1:] == (B, S) else position_ids.expand(-1, B, S)
-
-
 def _rotate(q, k, position_ids, plan, inverse):
-    given = [t for t in (q, k) if t is not None]
-    if not given:
+    first = k if q is None else q
+    if first is None:
         raise ValueError("rotary_axes: neither q nor k given")
-    first = given[0]
-    if not first.is_cuda:
-        raise RuntimeError("coat_amd kernels need tensors on the GPU (got a %s tensor)" % first.device.type)
-    for t in given:
-        if t.dim() != 4 or t.shape[:2] != first.shape[:2] or t.shape[3] != plan.head_dim:
-            raise ValueError(f"rotary_axes: expected [batch, seq, heads, {plan.head_dim}] tensors of one batch, got {tuple(t.shape)}")
-        if t.dtype != first.dtype or t.device != first.device:
-            raise ValueError("rotary_axes: q and k must have one dtype and device")
-    B, S, _, D = first.shape
-    device = first.device
-    pos = _positions(position_ids, plan, B, S, device)
-    turns, axis = plan.tables(device)
-    args, outs, kept = [], [], []
-    for t in (q, k):
-        if t is None:
-            args += (None, None, 0, 0, 0, 0)
-            outs.append(None)
-            continue
-        if t.stride(3) != 1:
-            t = t.contiguous()
-        kept.append(t)
-        out = torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
-        outs.append(out)
-        args += (t.data_ptr(), out.data_ptr(), *t.stride()[:3], t.shape[2])
-    _hip.launch("coat_rope_axes", first.get_device(), *args, _hip.dt(first), pos.data_ptr(), *pos.stride(), len(plan.sections),
-                turns.data_ptr(), axis.data_ptr(), plan.turning, D, plan.pairs, inverse, B, S, what="rotary_axes")
-    return outs[0], outs[1]
+    turns, axis = plan.tables(first.device)
+    return _hip.native().rotary_axes(q, k, position_ids, turns, axis, plan.head_dim, len(plan.sections), plan.turning, plan.pairs, inverse)
 
 
 def rotary_axes_forward(q, k, position_ids, plan):

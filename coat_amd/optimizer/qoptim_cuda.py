@@ -8,7 +8,6 @@ torch tensors in, everything updated in place; the work is done by libcoat_hip.s
 stream (the reference launches on the legacy default stream).  Errors the reference raises through
 AT_ASSERTM surface as RuntimeError with the same message."""
 import ctypes
-from array import array
 
 import torch
 
@@ -130,37 +129,6 @@ def fp8_adamw_step_multi(params, grads, exp_avg, scale_exp_avg, exp_avg_sq, scal
 
 
 # ------------------------------------------------------------------------------------------------ 32-bit states, clipping
-_dtype_of = torch.Tensor.dtype.__get__  # without a Python frame per tensor
-
-
-def _columns(what, lists):
-    """Checks parallel lists of tensors (name, tensors, dtype of all or None) that a multi-tensor call reads or writes flat: one
-    length, one device, equal sizes, contiguous.  Returns (device index, sizes, addresses of each list), the latter two as host arrays
-    that an entry point can read."""
-    first = lists[0][1]
-    n, index, T = len(first), first[0].get_device(), torch.Tensor
-    if index < 0:
-        raise RuntimeError(f"{what}: tensors must be on the GPU")
-    numel, out = array("q", map(T.numel, first)), []
-    for name, tensors, dtype in lists:
-        if len(tensors) != n:
-            raise RuntimeError(f"{what}: the tensor lists differ in length")
-        if set(map(T.get_device, tensors)) != {index}:
-            raise RuntimeError(f"{what}: {name} holds tensors that are not on the first tensor's device")
-        if dtype is not None and set(map(_dtype_of, tensors)) != {dtype}:
-            raise RuntimeError(f"{what}: {name} must all be {dtype}")
-        if tensors is not first and array("q", map(T.numel, tensors)) != numel:
-            raise RuntimeError(f"{what}: sizes of {name} differ from those of {lists[0][0]}")
-        if not all(map(T.is_contiguous, tensors)):
-            raise RuntimeError(f"{what}: {name} must be contiguous")
-        out.append(array("Q", map(T.data_ptr, tensors)))
-    return index, numel, out
-
-
-def _address(host_array):
-    return host_array.buffer_info()[0]
-
-
 def grad_norm_multi(grads, max_norm=None):
     """The 2-norm of all ``grads`` (fp32 / bf16 / fp16 GPU tensors) taken together, and the factor that clips them to ``max_norm``.
 
@@ -173,20 +141,7 @@ def grad_norm_multi(grads, max_norm=None):
         raise ValueError(f"grad_norm_multi: invalid max_norm {max_norm}")
     if not grads:
         raise ValueError("grad_norm_multi: no gradients")
-    if not all(map(torch.Tensor.is_contiguous, grads)):
-        grads = [g.contiguous() for g in grads]
-    n = len(grads)
-    index, numel, (addresses,) = _columns("grad_norm_multi", [("grads", grads, None)])
-    kinds = set(map(_dtype_of, grads))
-    dtypes = array("i", [_hip.dt(k) for k in kinds] * n if len(kinds) == 1 else [_hip.dt(g) for g in grads])
-    parts = _hip.lib().coat_grad_norm_partials(n, _address(numel))
-    if parts < 0:
-        _hip.check(parts, "grad_norm_multi")
-    work = grads[0].new_empty(max(parts, 1), dtype=torch.float64)
-    out = grads[0].new_empty(2, dtype=torch.float32)
-    _hip.launch("coat_grad_norm_multi", index, n, _address(addresses), _address(dtypes), _address(numel),
-                0.0 if max_norm is None else float(max_norm), work.data_ptr(), parts, out.data_ptr(), what="grad_norm_multi")
-    norm, scale = out.unbind()
+    norm, scale = _hip.native().grad_norm_multi(grads, 0.0 if max_norm is None else float(max_norm)).unbind()
     return norm, None if max_norm is None else scale
 
 
@@ -196,37 +151,6 @@ def adamw_step_multi(params, grads, exp_avg, exp_avg_sq, beta1, beta2, lr, wd, e
     they are stepped, and the parameters receive their rounding.  ``grad_scale``: a one-element fp32 tensor on the device that the
     gradients are multiplied by (``grad_norm_multi``).  ``step`` counts from 1 and is read on the host: a captured graph keeps it.
     Tensors that are stepped may share no memory with each other or with the gradients (RuntimeError)."""
-    n = len(params)
-    if n == 0:
+    if len(params) == 0:
         return
-    lists = [("params", params, params[0].dtype), ("grads", grads, grads[0].dtype if len(grads) else None),
-             ("exp_avg", exp_avg, torch.float32), ("exp_avg_sq", exp_avg_sq, torch.float32)]
-    if masters is not None:
-        lists.append(("masters", masters, torch.float32))
-    index, numel, addresses = _columns("adamw_step_multi", lists)
-    pdt, gdt = params[0].dtype, grads[0].dtype
-    if gdt != pdt and gdt != torch.float32:
-        raise RuntimeError(f"adamw_step_multi: grads dtype {gdt} is neither the params' {pdt} nor torch.float32")
-    if masters is not None and pdt == torch.float32:
-        raise RuntimeError("adamw_step_multi: masters are for parameters of 16 bits")
-    if n > 76:  # more than one launch: the library compares the tensors of each
-        written = addresses[0]
-        for column in addresses[2:]:
-            written = written + column
-        if len(set(written)) != len(written):  # empty tensors share the address 0
-            written = [a for a, size in zip(written, numel * (len(addresses) - 1)) if size]
-            if len(set(written)) != len(written):
-                raise RuntimeError("adamw_step_multi: a tensor that is stepped is given twice")
-    if not int(step) >= 1:
-        raise ValueError(f"adamw_step_multi: invalid step {step}")
-    if grad_scale is not None:
-        _check_grad_scale("adamw_step_multi", grad_scale, index)
-    p, g, m, v, w = (*map(_address, addresses), None)[:5]
-    hyper = array("d", (beta1, beta2, lr, wd, eps))
-    _hip.launch("coat_adamw_step_multi", index, n, p, _hip.dt(pdt), g, _hip.dt(gdt), m, v, w, _address(numel), _address(hyper),
-                int(step), None if grad_scale is None else grad_scale.data_ptr(), what="adamw_step_multi")
-    # written behind autograd's back: graphs that saved them must notice
-    try:
-        torch.autograd.graph.increment_version(params)
-    except RuntimeError:  # inference tensors have no version
-        torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+    _hip.native().adamw_step_multi(params, grads, exp_avg, exp_avg_sq, masters, beta1, beta2, lr, wd, eps, int(step), grad_scale)
