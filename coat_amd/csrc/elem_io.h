@@ -55,47 +55,23 @@ template <int DT, bool STREAM = false> __device__ __forceinline__ Raw8<DT> load_
     }
     return r;
 }
-// The same for a load that is issued well before its use: the last piece of a row is read as the eight elements that end the row,
-// and settle_row8 moves them to their places when they are used.  (Picking single elements needs their values, that is a wait
-// right after the load: one lane of a block then holds up every row, 1.8x the time at 4100 columns.)
-template <int DT, bool STREAM> __device__ __forceinline__ Raw8<DT> load_row8(const void* row, int c, int n, bool valid) {
+// A row of n elements in pieces of eight: the last piece of a row whose length is not a multiple of 8 is the eight elements that
+// end the row, so that every piece is one wide load and one wide store.  Elements that two pieces hold are computed and stored
+// twice, with the same value; sums count them in the first (own_element).  Rows of fewer than eight elements are one short piece.
+// (Element-wise ends cost much more: picking single elements waits for their load at once, which holds up every row of a block.)
+__device__ __forceinline__ int piece_begin(int c, int n) { return c + 8 <= n || n < 8 ? c : n - 8; }
+// Whether element j of the piece at piece_begin(c, n) belongs to column c + 0 .. 7 of the row, and not to the piece before.
+__device__ __forceinline__ bool own_element(int c, int n, int j) { return n >= 8 ? j >= c + 8 - n : j < n; }
+// RAGGED: n need not be a multiple of 8.  Otherwise c is below n only where a whole piece is.  Zeros if not valid or past the row.
+template <int DT, bool RAGGED, bool STREAM> __device__ __forceinline__ Raw8<DT> load_piece(const void* row, int c, int n, bool valid = true) {
     Raw8<DT> r;
 #pragma unroll
     for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = 0;
     if (valid && c < n) {
-        if (n >= 8) {
-            r = load_raw8<DT, STREAM>(elem_at<DT>(row, c + 8 <= n ? c : n - 8), 8);
-        } else {
-            r = load_raw8<DT>(elem_at<DT>(row, c), n - c);
-        }
+        if (!RAGGED || n >= 8) r = load_raw8<DT, STREAM>(elem_at<DT>(row, RAGGED ? piece_begin(c, n) : c), 8);
+        else r = load_raw8<DT>(row, n);
     }
     return r;
-}
-// RAGGED: n need not be a multiple of 8.  Otherwise c is below n only where a whole piece is.
-template <int DT, bool RAGGED, bool STREAM> __device__ __forceinline__ Raw8<DT> load_piece(const void* row, int c, int n, bool valid = true) {
-    if (RAGGED) return load_row8<DT, STREAM>(row, c, n, valid);
-    Raw8<DT> r;
-#pragma unroll
-    for (int k = 0; k < (DT == kF32 ? 8 : 4); k++) r.w[k] = 0;
-    if (valid && c < n) r = load_raw8<DT, STREAM>(elem_at<DT>(row, c), 8);
-    return r;
-}
-template <int DT> __device__ __forceinline__ void settle_row8(Raw8<DT>& r, int c, int n) {
-    const int past = c + 8 - n;  // elements of this piece past the end of the row
-    if (past > 0 && past < 8 && n >= 8) {
-        constexpr int W = DT == kF32 ? 8 : 4;
-        if (DT != kF32 && (past & 1)) {
-#pragma unroll
-            for (int k = 0; k < W; k++) r.w[k] = r.w[k] >> 16 | (k + 1 < W ? r.w[(k + 1) % W] << 16 : 0u);
-        }
-        const int words = past >> (DT == kF32 ? 0 : 1);
-#pragma unroll
-        for (int d = 1; d < 8; d <<= 1)
-            if (words & d) {
-#pragma unroll
-                for (int k = 0; k < W; k++) r.w[k] = k + d < W ? r.w[(k + d) % W] : 0u;
-            }
-    }
 }
 template <int DT> __device__ __forceinline__ void raw8_to_f32(const Raw8<DT>& r, float* o) {
     if (DT == kF32) {

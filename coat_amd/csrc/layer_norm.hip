@@ -34,7 +34,7 @@ template <int W> __device__ __forceinline__ float block_sum(float v, float* red)
 // lanes of a wave read one run of memory.  L = 8 .. 64: a wave works on 64 / L rows at a time and no barrier is needed.
 // L = kBlock: the block works on one row with as many waves as that takes.  The weights stay in registers over the rows of a
 // block, and the next row's loads are issued before the sums of the present one are exchanged.
-// RAGGED: N is not a multiple of 8; the last piece of a row is then incomplete.
+// RAGGED: N is not a multiple of 8; the last piece of a row then shares elements with the one before, which its sums leave out.
 constexpr int kBlock = 0;
 constexpr int form_threads(int L, int C) { return L != kBlock ? 256 : C <= 2 ? 1024 : 512; }  // launch bound
 constexpr int form_rows(int L) { return L != kBlock ? 256 / L : 1; }                          // rows at a time
@@ -76,16 +76,19 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __res
             wv[k][j] = 1.0f;
             bv[k][j] = 0.0f;
         }
-        if (w) load8_rt(w, w_dt, (k * lanes + l) * 8, N, wv[k]);
-        if (b) load8_rt(b, w_dt, (k * lanes + l) * 8, N, bv[k]);
+        const int c = (k * lanes + l) * 8, at = RAGGED ? piece_begin(c, N) : c;
+        if (w && c < N) load8_rt(w, w_dt, at, N, wv[k]);
+        if (b && c < N) load8_rt(b, w_dt, at, N, bv[k]);
     }
     for (int64_t i = 0; i < rounds; i++, row += step) {
         float v[C][8], s = 0.0f;
 #pragma unroll
         for (int k = 0; k < C; k++) {
-            if (RAGGED) settle_row8<DT>(raw[k], (k * lanes + l) * 8, N);
             raw8_to_f32<DT>(raw[k], v[k]);
-            s += ((v[k][0] + v[k][1]) + (v[k][2] + v[k][3])) + ((v[k][4] + v[k][5]) + (v[k][6] + v[k][7]));
+            float own[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) own[j] = !RAGGED || own_element((k * lanes + l) * 8, N, j) ? v[k][j] : 0.0f;
+            s += ((own[0] + own[1]) + (own[2] + own[3])) + ((own[4] + own[5]) + (own[6] + own[7]));
         }
         if (i + 1 < rounds) {
             const int64_t next = row + step;
@@ -97,11 +100,11 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __res
         s = 0.0f;
 #pragma unroll
         for (int k = 0; k < C; k++) {
-            const int left = N - (k * lanes + l) * 8;
+            const int c = (k * lanes + l) * 8;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 v[k][j] -= mean;
-                const float d = (RAGGED ? j : 0) < left ? v[k][j] : 0.0f;
+                const float d = c < N && (!RAGGED || own_element(c, N, j)) ? v[k][j] : 0.0f;
                 s = fmaf(d, d, s);
             }
         }
@@ -113,7 +116,7 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __res
                 if (c >= N) continue;
 #pragma unroll
                 for (int j = 0; j < 8; j++) v[k][j] = fmaf(v[k][j] * rstd, wv[k][j], bv[k][j]);
-                store8<DT>(elem_at<DT>(y, row * N + c), RAGGED ? N - c : 8, v[k]);
+                store8<DT>(elem_at<DT>(y, row * N + (RAGGED ? piece_begin(c, N) : c)), RAGGED ? N : 8, v[k]);
             }
             if (l == 0) {
                 mean_out[row] = mean;
@@ -169,17 +172,14 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
             wv[k][j] = 1.0f;
             aw[k][j] = ab[k][j] = 0.0f;
         }
-        if (w) load8_rt(w, w_dt, (k * lanes + l) * 8, N, wv[k]);
+        const int c = (k * lanes + l) * 8;
+        if (w && c < N) load8_rt(w, w_dt, RAGGED ? piece_begin(c, N) : c, N, wv[k]);
     }
     for (int64_t i = 0; i < rounds; i++, row += step) {
         if (kLean) load(row);
         float h[C][8], t[C][8], st = 0.0f, sth = 0.0f;
 #pragma unroll
         for (int k = 0; k < C; k++) {
-            if (RAGGED) {
-                settle_row8<DT>(rx[k], (k * lanes + l) * 8, N);
-                settle_row8<DT>(rg[k], (k * lanes + l) * 8, N);  // zeros past the end: they add nothing to any sum
-            }
             raw8_to_f32<DT>(rx[k], h[k]);
             raw8_to_f32<DT>(rg[k], t[k]);
 #pragma unroll
@@ -189,9 +189,10 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
                     aw[k][j] = fmaf(t[k][j], h[k][j], aw[k][j]);
                     ab[k][j] += t[k][j];
                 }
-                t[k][j] *= wv[k][j];
-                st += t[k][j];
-                sth = fmaf(t[k][j], h[k][j], sth);
+                t[k][j] *= wv[k][j];  // zeros past the row: they add nothing to any sum
+                const float own = !RAGGED || own_element((k * lanes + l) * 8, N, j) ? t[k][j] : 0.0f;
+                st += own;
+                sth = fmaf(own, h[k][j], sth);
             }
         }
         const float rs = rstd;
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
                     if (c >= N) continue;
 #pragma unroll
                     for (int j = 0; j < 8; j++) t[k][j] = (t[k][j] - fmaf(h[k][j], mth, mt)) * rs;
-                    store8<DT>(elem_at<DT>(dx, row * N + c), RAGGED ? N - c : 8, t[k]);
+                    store8<DT>(elem_at<DT>(dx, row * N + (RAGGED ? piece_begin(c, N) : c)), RAGGED ? N : 8, t[k]);
                 }
             }
         }
@@ -231,12 +232,14 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
 #pragma unroll
             for (int k = 0; k < C; k++) {
                 const int c = (k * lanes + l) * 8;
+                if (c >= N) continue;
+                const int at = RAGGED ? piece_begin(c, N) : c;
                 if (alone) {
-                    if (dw) store8_rt(dw, w_dt, c, N, aw[k]);
-                    if (db) store8_rt(db, w_dt, c, N, ab[k]);
+                    if (dw) store8_rt(dw, w_dt, at, N, aw[k]);
+                    if (db) store8_rt(db, w_dt, at, N, ab[k]);
                 } else {
-                    if (dw) store8<kF32>(pw + blockIdx.x * (int64_t)N + c, N - c, aw[k]);
-                    if (db) store8<kF32>(pb + blockIdx.x * (int64_t)N + c, N - c, ab[k]);
+                    if (dw) store8<kF32>(pw + blockIdx.x * (int64_t)N + at, N - at, aw[k]);
+                    if (db) store8<kF32>(pb + blockIdx.x * (int64_t)N + at, N - at, ab[k]);
                 }
             }
         } else {
@@ -247,9 +250,11 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
                 if (!out) continue;
                 __syncthreads();
 #pragma unroll
-                for (int k = 0; k < C; k++)
+                for (int k = 0; k < C; k++) {
+                    const int c = (k * lanes + l) * 8, at = RAGGED && c < N ? piece_begin(c, N) : c;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) cols[kShared ? r : 0][kShared ? (k * L + l) * 8 + j : 0] = which == 0 ? aw[k][j] : ab[k][j];
+                    for (int j = 0; j < 8; j++) cols[kShared ? r : 0][kShared ? at + j : 0] = which == 0 ? aw[k][j] : ab[k][j];
+                }
                 __syncthreads();
                 for (int c = threadIdx.x; c < N; c += 256) {
                     float s = cols[0][kShared ? c : 0];

@@ -41,7 +41,7 @@ struct RopeArgs {
 // n / d for n * d < 2^32, with m = ceil(2^32 / d)
 __device__ __forceinline__ uint32_t div_magic(uint32_t n, uint32_t d, uint32_t m) { return d == 1 ? n : __umulhi(n, m); }
 
-// WHOLE: every piece is complete (pairs and head_dim multiples of 8), no element-wise ends.
+// WHOLE: pairs and the rest are multiples of 8.
 template <int DT, bool ADJ, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rope_axes(RopeArgs A) {
     __shared__ float2 cs[kRopeSlots];
@@ -75,6 +75,7 @@ __global__ __launch_bounds__(256) void k_rope_axes(RopeArgs A) {
         J.n = rest ? A.head_dim - rot : ADJ ? rot : A.pairs;
         J.a = load_piece<DT, !WHOLE, true>(rest ? elem_at<DT>(x, rot) : x, J.e, J.n);
         if (!ADJ && !rest) J.b = load_piece<DT, !WHOLE, true>(elem_at<DT>(x, A.pairs), J.e, J.n);
+        if (!WHOLE) J.e = piece_begin(J.e, J.n);
         return J;
     };
     Job J;
@@ -90,14 +91,10 @@ __global__ __launch_bounds__(256) void k_rope_axes(RopeArgs A) {
     }
     __syncthreads();
     for (int job = threadIdx.x; job < jobs;) {
-        const int e = J.e, left = WHOLE ? 8 : J.n - e, piece = J.piece;
+        const int e = J.e, left = WHOLE ? 8 : J.n, piece = J.piece;  // fewer than 8 only where the whole run is
         void* y = J.y;
         const float2* c = cs + J.token * A.pairs;
         float u[8], v[8];
-        if (!WHOLE) {
-            settle_row8<DT>(J.a, e, J.n);
-            if (!ADJ) settle_row8<DT>(J.b, e, J.n);
-        }
         raw8_to_f32<DT>(J.a, u);
         if (!ADJ) raw8_to_f32<DT>(J.b, v);
         job += 256;
