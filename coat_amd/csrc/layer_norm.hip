@@ -126,8 +126,8 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __res
     }
 }
 
-// x and dy are not needed again after this kernel: streaming loads ([262144, 128] bf16: 42 -> 39 us with the sums; no difference at
-// 4096 columns; in the forward, whose x the backward reads, 24 -> 26).
+// x and dy are not needed again after this kernel: streaming loads ([262144, 128] bf16: 42 -> 39 us with the sums; with the caches
+// full of another kernel's writes 44 against 68; in the forward, whose x the backward reads, 24 -> 26).
 // dx, and with SUMS the sums for dw and db (either may be NULL): one partial row per block, in pw / pb, or, if there is one block
 // only, dw and db themselves.
 template <int DT, int L, int C, bool RAGGED, bool SUMS>

@@ -125,6 +125,24 @@ def test_adamw_step_entry(L, p):
     assert b"shares memory" in L.coat_status_string(EOVERLAP)
 
 
+def test_binding_is_built_for_this_library_and_refuses_other_objects():
+    from coat_amd import _hip
+    native = _hip.native()
+    assert native is _hip.native() and native.ABI_VERSION == _hip.ABI_VERSION
+    t = torch.zeros(4, 8)
+    for call in (lambda: native.layer_norm_forward(3, None, None, 1e-5), lambda: native.layer_norm_forward(t, [1.0], None, 1e-5),
+                 lambda: native.layer_norm_forward(t, None, None, "eps"), lambda: native.layer_norm_forward(t),
+                 lambda: native.grad_norm_multi([t, 3], 1.0), lambda: native.grad_norm_multi(3, 1.0),
+                 lambda: native.adamw_step_multi([t], [t], [t], [None], None, 0.9, 0.9, 0.1, 0.1, 1e-8, 1, None),
+                 lambda: native.rotary_axes(None, 3, t, t, t, 8, 1, 4, False, False)):
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(ValueError):
+        native.bind({}, torch.cuda.current_stream)
+    with pytest.raises(RuntimeError, match="GPU"):  # and still holds the library
+        native.layer_norm_forward(t, None, None, 1e-5)
+
+
 def test_python_refusals():
     from coat_amd.activation.norm import layer_norm, layer_norm_forward
     from coat_amd.models.rotary import RotaryAxes, rotary_axes, rotary_axes_forward
