@@ -69,11 +69,21 @@ template <int DT> __device__ __forceinline__ double sumsq_chunk(const void* g, i
                 if (DT != kF32) s = fma(b, b, s);
             }
     } else {  // the tensor's last chunk
-        for (int64_t e = begin + threadIdx.x * 8; e < numel; e += 2048) {
-            float v[8];
-            load8<DT>(elem_at<DT>(g, e), numel - e, v);
+        const int n = (int)(numel - begin);
+        const void* p = elem_at<DT>(g, begin);
+        Raw8<DT> r[kNormChunk / 2048];
 #pragma unroll
-            for (int i = 0; i < 8; i++) s = fma((double)v[i], (double)v[i], s);
+        for (int j = 0; j < kNormChunk / 2048; j++) r[j] = load_piece<DT, true, true>(p, j * 2048 + threadIdx.x * 8, n);
+#pragma unroll
+        for (int j = 0; j < kNormChunk / 2048; j++) {
+            const int c = j * 2048 + threadIdx.x * 8;
+            float v[8];
+            raw8_to_f32<DT>(r[j], v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const double a = c < n && own_element(c, n, i) ? v[i] : 0.0f;
+                s = fma(a, a, s);
+            }
         }
     }
     return s;

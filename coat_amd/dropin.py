@@ -13,8 +13,8 @@ def install():
     sys.modules.setdefault("qoptim_cuda", _qoptim)
     sys.modules.setdefault("coat", coat_amd)
     for info in pkgutil.walk_packages(coat_amd.__path__, prefix="coat_amd."):
-        if info.name in ("coat_amd.dropin", "coat_amd.build") or info.name.endswith("libcoat_hip"):
-            continue  # the C-ABI shared object sits in the package directory but is not a Python module
+        if info.name in ("coat_amd.dropin", "coat_amd.build") or info.name.endswith(("libcoat_hip", "_binding")):
+            continue  # the shared objects sit in the package directory: the C ABI is no Python module, the binding no interface
         mod = importlib.import_module(info.name)
         sys.modules.setdefault("coat" + info.name[len("coat_amd"):], mod)
 

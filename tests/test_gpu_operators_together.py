@@ -309,3 +309,67 @@ def test_training_step_captured_and_replayed(dev):
         for k in eager:
             for a, e in zip(*[t if isinstance(t, list) else [t] for t in (graphed[k], eager[k])]):
                 assert torch.equal(a, e), (seed, k)
+
+
+def test_autograd_of_rotary_and_norm_captured_and_replayed(dev):
+    """Forward and backward through autograd inside one capture, with leaves of the graph's own; eager runs on other leaves."""
+    from coat_amd.activation.norm import layer_norm
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes
+    plan = RotaryAxes(64, (8, 12, 12))
+
+    def run(x, w, b, pos, g):
+        q, k = rotary_axes(x, x[:, :, :2], pos, plan)
+        y = layer_norm(torch.cat((q, k), 2).flatten(2), w, b)
+        return (y, *torch.autograd.grad(y, (x, w, b), g))
+
+    def inputs(seed):
+        return [randn(dev, seed, 2, 30, 4, 64, dtype=torch.bfloat16).requires_grad_(), (1 + randn(dev, seed + 1, 384, scale=0.1)).requires_grad_(),
+                randn(dev, seed + 2, 384).requires_grad_(), torch.randint(0, 99, (3, 2, 30), generator=torch.Generator().manual_seed(seed)).to(dev),
+                randn(dev, seed + 3, 2, 30, 384, dtype=torch.bfloat16)]
+
+    static = inputs(1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(*static)
+    for seed in (10, 20, 30):
+        new = inputs(seed)
+        with torch.no_grad():
+            for a, e in zip(static, new):
+                a.copy_(e)
+        graph.replay()
+        want = run(*new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, e) for a, e in zip(out, want)), seed
+
+
+def test_two_threads_on_streams_of_their_own(dev):
+    import threading
+
+    from coat_amd.activation.norm import layer_norm_backward, layer_norm_forward
+    from coat_amd.optimizer import qoptim_cuda
+
+    def work(seed):
+        x, w = randn(dev, seed, 300, 1001, dtype=torch.bfloat16), randn(dev, seed + 1, 1001)
+        m, v = torch.zeros_like(w), torch.zeros_like(w)
+        for n in range(1, 20):
+            y, mean, rstd = layer_norm_forward(x, w, w)
+            dx, dw, db = layer_norm_backward(y, x, mean, rstd, w)
+            norm, scale = qoptim_cuda.grad_norm_multi([dw, db], 1.0)
+            qoptim_cuda.adamw_step_multi([w], [dw], [m], [v], *HYPER, n, grad_scale=scale)
+        return y, dx, w, m, v, norm
+
+    want, got = [work(1), work(50)], [None, None]
+    torch.cuda.synchronize()
+
+    def thread(i, seed):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = work(seed)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=thread, args=(i, s)) for i, s in enumerate((1, 50))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, e in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, e))

@@ -63,7 +63,7 @@ def test_rope_axes_entry(L, p):
     for bad in (dict(batch=-1), dict(seq=-1), dict(heads=-1), dict(kheads=-1), dict(axes=0), dict(pairs=0), dict(dim=1), dict(adjacent=2),
                 dict(inverse=2), dict(q=None), dict(qo=None), dict(k=None), dict(ko=None), dict(pos=None), dict(turns=None), dict(axis=None)):
         assert rope(L, p, **bad) == EINVAL, bad
-    for bad in (dict(pairs=17), dict(dim=2049), dict(heads=1025), dict(kheads=1025), dict(batch=1 << 40, seq=1)):
+    for bad in (dict(pairs=17), dict(dim=2049), dict(heads=1025), dict(kheads=1025), dict(batch=1 << 40, seq=1), dict(batch=1 << 40, seq=1 << 40)):
         assert rope(L, p, **bad) == ESHAPE, bad
     for bad in (dict(q=p + 2), dict(ko=p + 1), dict(pos=p + 4), dict(turns=p + 4), dict(axis=p + 2)):
         assert rope(L, p, **bad) == EALIGN, bad
