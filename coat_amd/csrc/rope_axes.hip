@@ -139,8 +139,8 @@ extern "C" int coat_rope_axes(const void* q, void* q_out, int64_t q_sb, int64_t 
     if (batch == 0 || seq == 0 || q_heads + k_heads == 0) return COAT_OK;
     if (batch > ((int64_t)1 << 40) / seq) return COAT_ESHAPE;
     if ((q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)) || !pos || !turns || !axis) return COAT_EINVAL;
-    const uintptr_t mask = dtype == COAT_F32 ? 3 : 1;
-    if ((((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)k_out) & mask) || (((uintptr_t)pos | (uintptr_t)turns) & 7) ||
+    const uintptr_t mask = dtype == COAT_F32 ? 3 : 1, at_q = (uintptr_t)q | (uintptr_t)q_out, at_k = (uintptr_t)k | (uintptr_t)k_out;
+    if ((q_heads && (at_q & mask)) || (k_heads && (at_k & mask)) || (((uintptr_t)pos | (uintptr_t)turns) & 7) ||
         ((uintptr_t)axis & 3))
         return COAT_EALIGN;
     RopeArgs A;

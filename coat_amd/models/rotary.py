@@ -47,6 +47,8 @@ class RotaryAxes:
         position_ids [axes, B, S]."""
         if self.pairs or 2 * self.turning != self.head_dim:
             raise ValueError("RotaryAxes.cos_sin: only for heads that turn whole, in the (j, j + P) layout")
+        if position_ids.dim() != 3 or position_ids.shape[0] != len(self.sections):
+            raise ValueError(f"RotaryAxes: expected position_ids of shape [{len(self.sections)}, batch, seq], got {list(position_ids.shape)}")
         freq = torch.tensor(self._freq, dtype=torch.float64, device=position_ids.device)
         angle = position_ids[torch.tensor(self._axis, device=position_ids.device)].permute(1, 2, 0).double() * freq
         angle = torch.cat((angle, angle), -1)
@@ -84,6 +86,7 @@ class _RotaryAxes(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dq, dk):
+        dq, dk = (g if needed else None for g, needed in zip((dq, dk), ctx.needs_input_grad))
         if dq is None and dk is None:
             return None, None, None, None
         (position_ids,) = ctx.saved_tensors

@@ -50,8 +50,8 @@ enum coat_fp8 { COAT_E4M3 = 0, COAT_E5M2 = 1 }; /* torch.float8_e4m3fn / torch.f
  * argument became COAT_MAX_WORDS words; 3: coat_fp8_gemm_residual, coat_fp8_rmsnorm_backward_add and coat_attention_forward_bf16 added,
  * coat_hbm_probe removed; 4: coat_rope_bf16 and coat_attention_forward_bf16 take a maximum buffer, the multi-tensor optimizer
  * steps and coat_fp8_layernorm_backward_add added; 5: coat_fp8_quantize_perblock added;
- * 6: coat_layer_norm_*, coat_rope_axes, coat_grad_norm_*, coat_adamw_step_multi and the _scaled multi-tensor steps added).  A caller compiled against this header checks coat_abi_version() == COAT_ABI_VERSION when it
- * loads the library. */
+ * 6: coat_layer_norm_*, coat_rope_axes, coat_grad_norm_*, coat_adamw_step_multi and the _scaled multi-tensor steps added).  A caller
+ * compiled against this header checks coat_abi_version() == COAT_ABI_VERSION when it loads the library. */
 #define COAT_ABI_VERSION 6
 int coat_abi_version(void);
 const char* coat_version(void);
@@ -312,8 +312,8 @@ int coat_layer_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const v
 int coat_layer_norm_partials(int64_t M, int64_t N);
 /* dx (dense, x_dtype), dw and db (w_dtype), each optional (NULL).  dy, x of x_dtype with row pitches (0 = N).  partial: fp32
  * workspace [2, n_partial, N] if both dw and db are wanted, [1, n_partial, N] for one, unused for none; 1 <= n_partial <= 65535
- * blocks (with one, partial may be NULL for N <= 16384) each sum their rows into one partial row, which are then added in a fixed order: the same bits every time for one
- * n_partial.  M = 0 gives zero gradients. */
+ * blocks (with one, partial may be NULL for N <= 16384) each sum their rows into one partial row, which are then added in a fixed
+ * order: the same bits every time for one n_partial.  M = 0 gives zero gradients. */
 int coat_layer_norm_backward(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, int x_dtype, const float* mean,
                              const float* rstd, const void* w, int w_dtype, void* dx, void* dw, void* db, float* partial,
                              int n_partial, int64_t M, int64_t N, void* stream);
@@ -432,9 +432,8 @@ int coat_grad_norm_multi(int count, const void* const* grads, const int* dtypes,
 /* AdamW step of several tensors with both moments in fp32, 76 tensors to a launch; the formula of coat_fp8_adamw_step_multi.
  * params of p_dtype; grads of p_dtype or fp32; masters NULL, or fp32 copies of 16-bit parameters that are stepped instead, the
  * parameter receiving their rounding.  hyper: host array of five doubles: beta1, beta2 (both in [0, 1)), lr, weight decay,
- * eps.  grad_scale: NULL,
- * or one fp32 in device memory that the gradients are multiplied by (out[1] above).  Host arrays are read before the call
- * returns; addresses need the element's own alignment only; a tensor that is written may share no memory with another
+ * eps.  grad_scale: NULL, or one fp32 in device memory that the gradients are multiplied by (out[1] above).  Host arrays are
+ * read before the call returns; addresses need the element's own alignment only; a tensor that is written may share no memory with another
  * tensor (COAT_EOVERLAP where two of one launch do); empty ones are skipped; everything is checked before the first launch. */
 int coat_adamw_step_multi(int count, void* const* params, int p_dtype, const void* const* grads, int g_dtype, float* const* exp_avg,
                           float* const* exp_avg_sq, float* const* masters, const int64_t* numel, const double* hyper, int step,

@@ -34,7 +34,7 @@ def rotated(x, pos, sections, theta, restart, pairs, sign=1.0):
 
 def check(x, got, pos, plan, sign=1.0):
     want, size = rotated(x, pos, plan.sections, plan.theta, plan.restart, plan.pairs, sign)
-    bound = torch.finfo(x.dtype).eps / 2 * want.abs() + 5e-7 * size + torch.finfo(x.dtype).tiny * (size > 0)
+    bound = torch.finfo(x.dtype).eps / 2 * want.abs() + 5e-7 * size + torch.finfo(x.dtype).tiny * torch.finfo(x.dtype).eps / 2 * (size > 0)
     err = (got.double() - want).abs()
     assert got.shape == x.shape and got.dtype == x.dtype and got.is_contiguous()
     assert (err <= bound).all(), (err - bound).max()
@@ -175,6 +175,25 @@ def test_autograd_and_differences(dev):
     assert torch.equal(q.grad, want[0])
     out, none = rotary_axes(q, None, pos, plan)
     assert none is None and torch.equal(out, qo)
+    q.grad, fixed = None, k.detach()
+    qo, ko = rotary_axes(q, fixed, pos, plan)  # k is no leaf of the graph
+    torch.autograd.backward((qo, ko), (gq, gk))
+    assert torch.equal(q.grad, want[0]) and fixed.grad is None
+
+
+def test_c_entry_ignores_the_pointers_of_no_heads(dev):
+    from coat_amd import _hip
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes_forward
+    plan = RotaryAxes(32, (8, 8))
+    x, pos = randn(dev, 7, 2, 5, 3, 32), positions(dev, 8, 2, 2, 5, 100)
+    turns, axis = plan.tables(x.device)
+    want, out = rotary_axes_forward(x, None, pos, plan)[0], torch.empty_like(x)
+    one, none = (x.data_ptr(), out.data_ptr(), 5 * 96, 96, 32, 3), (1, 3, 0, 0, 0, 0)
+    for args in (one + none, none + one):
+        out.zero_()
+        assert _hip.lib().coat_rope_axes(*args, _hip.F32, pos.data_ptr(), 10, 5, 1, 2, turns.data_ptr(), axis.data_ptr(), 16, 32, 0, 0, 2, 5,
+                                         _hip.stream(x.device)) == 0
+        assert torch.equal(out, want)
 
 
 def test_another_stream_and_a_graph(dev):

@@ -245,6 +245,11 @@ def test_optimizer_refusals():
     for bad in (dict(state_bits=4), dict(master_weights=True)):
         with pytest.raises(ValueError):
             CoatAdamW([dict(params=[w], **bad)])
+    for kw in (dict(), dict(max_grad_norm=1.0)):  # one norm for all groups
+        with pytest.raises(ValueError, match="max_grad_norm"):
+            CoatAdamW([dict(params=[w], max_grad_norm=0.5)], **kw)
+    again = CoatAdamW([w], max_grad_norm=1.0)
+    assert CoatAdamW(again.param_groups, max_grad_norm=1.0).param_groups[0]["max_grad_norm"] == 1.0
     opt = CoatAdamW([w])  # the reference's groups are unchanged where nothing is asked for
     assert set(opt.param_groups[0]) == {"params", "lr", "betas", "eps", "weight_decay", "amsgrad", "fused"}
     assert CoatAdamW([w], state_bits=32, max_grad_norm=0.0).param_groups[0]["state_bits"] == 32
@@ -269,5 +274,8 @@ def test_attention_module_evaluates_several_axes_on_the_cpu():
     rq, rk = apply_rotary_pos_emb(heads[0], heads[1], ang.cos(), ang.sin())
     s = (rq @ rk.transpose(2, 3) / 32 ** 0.5).masked_fill(torch.triu(torch.ones(7, 7, dtype=torch.bool), 1), float("-inf")).softmax(-1)
     assert torch.allclose(out.double(), (s @ heads[2]).transpose(1, 2).reshape(1, 7, 64), rtol=0, atol=1e-5)
+    for bad in (pos[:2], torch.cat((pos, pos))):
+        with pytest.raises(ValueError, match="position_ids"):
+            module(q, k, v, position_ids=bad)
     with pytest.raises(ValueError, match="rotary_sections"):
         LlamaSdpaAttentionWithoutLinear(CoatLlamaConfig(hidden_size=64, num_attention_heads=2))(q, k, v, position_ids=pos)
