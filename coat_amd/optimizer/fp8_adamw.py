@@ -47,9 +47,11 @@ class CoatAdamW(Optimizer):
         max_grad_norm: Optional[float] = None,
     ):
         """``state_bits=32`` keeps both moments in fp32 (norm weights, embeddings); ``master_weights`` then also an fp32 copy of
-        16-bit parameters (state key ``master``).  Both may be given per parameter group.  ``max_grad_norm``: the gradients of
-        all groups are clipped to that global 2-norm inside the step (``grad_norm`` then holds the norm of the last step, on the
-        device; the gradients themselves stay as they are).  None of the three is in the reference."""
+        16-bit parameters (state key ``master``), made at the first step: what is written into the parameters from outside after
+        that is lost at the next one.  Both may be given per parameter group.  ``max_grad_norm``: the gradients of all groups, on
+        one device, are clipped to that global 2-norm of this process's gradients inside the step (``grad_norm`` then holds the
+        norm of the last step, on the device; the gradients themselves stay as they are).  None of the three is in the
+        reference."""
         # multi_tensor (not in the reference): parameters of one dtype, device and step count share kernel launches
         self.multi_tensor = multi_tensor
         self.qargs = QuantizationConfig() if qargs is None else qargs
@@ -85,6 +87,9 @@ class CoatAdamW(Optimizer):
             raise ValueError(f"Invalid state_bits: {bits} (8 or 32)")
         if param_group.get("master_weights", self.defaults.get("master_weights", False)) and bits != 32:
             raise ValueError("master_weights needs state_bits=32")
+        clip = self.defaults.get("max_grad_norm")
+        if param_group.get("max_grad_norm", clip) != clip:
+            raise ValueError("max_grad_norm is one for all parameter groups")
         super().add_param_group(param_group)
 
     # ------------------------------------------------------------------ state
