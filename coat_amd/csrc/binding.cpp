@@ -8,10 +8,14 @@
 // Errors: ValueError and RuntimeError as the rest of the package raises them; nothing is launched before everything is checked.
 #include <Python.h>
 
+#include <ATen/TracerMode.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -66,6 +70,25 @@ int64_t whole(PyObject* o) {
 void arguments(const char* who, Py_ssize_t got, Py_ssize_t wanted) {
     TORCH_CHECK_TYPE(got == wanted, who, ": ", wanted, " arguments are needed, got ", got);
     TORCH_CHECK(raw_stream, who, ": the binding has no library yet");
+}
+
+// torch does not see what is computed here: a forward-mode tangent would be lost and read as a zero derivative, a recorded program would
+// return memory that nothing fills.  Both are refused.  Inside an autograd function, where torch turns forward mode off, they are that
+// function's concern (it refuses tangents itself and is recorded as one step), but for a recording of dispatched operations, which
+// goes through it.
+bool forward_mode() {
+    return c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::ForwardADLevel::try_get_by_idx(0);
+}
+void no_tangent(const at::Tensor& t, const char* who) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), who, ": forward-mode derivatives are not implemented");
+}
+void unrecorded(const char* who, std::initializer_list<const at::Tensor*> tensors) {
+    const bool recorded = c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() ||
+                          (at::tracer::impl::is_dispatch_enabled() && c10::AutogradState::get_tls_state().get_fw_grad_mode());
+    TORCH_CHECK_NOT_IMPLEMENTED(!recorded, who, ": a trace cannot record this call");
+    if (forward_mode())
+        for (const at::Tensor* t : tensors)
+            if (t) no_tangent(*t, who);
 }
 
 const char* name_of(at::ScalarType t) {
@@ -162,6 +185,7 @@ PyObject* layer_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor& x = tensor(a[0], who, "x");
     const at::Tensor *w = tensor_or_none(a[1], who, "weight"), *b = tensor_or_none(a[2], who, "bias");
     const double eps = real(a[3]);
+    unrecorded(who, {&x, w, b});
     norm_arguments(who, x, w, b);
     TORCH_CHECK_VALUE(eps >= 0.0, who, ": invalid eps ", eps);
     const c10::DeviceGuard guard(x.device());
@@ -184,6 +208,7 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     arguments(who, n, 8);
     const at::Tensor &dy = tensor(a[0], who, "dy"), &x = tensor(a[1], who, "x"), &mean = tensor(a[2], who, "mean"), &rstd = tensor(a[3], who, "rstd");
     const at::Tensor* w = tensor_or_none(a[4], who, "weight");
+    unrecorded(who, {&dy, &x, &mean, &rstd, w});
     norm_arguments(who, x, w, nullptr);
     const int64_t N = x.size(-1), M = x.numel() / N;
     TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type() && dy.device() == x.device(), who,
@@ -225,6 +250,7 @@ PyObject* rotary_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor &turns = tensor(a[3], who, "turns"), &axis = tensor(a[4], who, "axis");
     const int64_t D = whole(a[5]), axes = whole(a[6]), pairs = whole(a[7]);
     TORCH_CHECK_VALUE(q || k, who, ": neither q nor k given");
+    unrecorded(who, {q, k});
     const at::Tensor& first = q ? *q : *k;
     on_gpu(first);
     for (const at::Tensor* t : {q, k}) {
@@ -292,6 +318,9 @@ PyObject* grad_norm_multi(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const double max_norm = real(a[1]);
     const Py_ssize_t count = grads.size();
     TORCH_CHECK_VALUE(count > 0, who, ": no gradients");
+    unrecorded(who, {});
+    if (forward_mode())
+        for (Py_ssize_t i = 0; i < count; i++) no_tangent(grads[i], who);
     const at::Device device = grads[0].device();
     on_gpu(grads[0]);
     const c10::DeviceGuard guard(device);
@@ -336,6 +365,11 @@ PyObject* adamw_step_multi(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Py_ssize_t count = params.size();
     TORCH_CHECK_VALUE(count > 0, who, ": no parameters");
     for (int c = 1; c < columns; c++) TORCH_CHECK(lists[c]->size() == count, who, ": the tensor lists differ in length");
+    const at::Tensor* scale = tensor_or_none(a[11], who, "grad_scale");
+    unrecorded(who, {scale});
+    if (forward_mode())
+        for (int c = 0; c < columns; c++)
+            for (Py_ssize_t i = 0; i < count; i++) no_tangent((*lists[c])[i], who);
     on_gpu(params[0]);
     const at::Device device = params[0].device();
     const at::ScalarType types[5] = {params[0].scalar_type(), grads[0].scalar_type(), at::kFloat, at::kFloat, at::kFloat};
@@ -359,7 +393,6 @@ PyObject* adamw_step_multi(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK(!masters || p_dtype != COAT_F32, who, ": masters are for parameters of 16 bits");
     const int64_t step = whole(a[10]);
     TORCH_CHECK_VALUE(step >= 1 && step <= INT32_MAX, who, ": invalid step ", step);
-    const at::Tensor* scale = tensor_or_none(a[11], who, "grad_scale");
     TORCH_CHECK(!scale || (scale->scalar_type() == at::kFloat && scale->numel() == 1 && scale->device() == device), who,
                 ": grad_scale must be one fp32 element on the parameters' device");
     if (count > 76) {  // more than one launch: the library compares the tensors of each

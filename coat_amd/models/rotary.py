@@ -94,7 +94,8 @@ class _RotaryAxes(torch.autograd.Function):
 
 
 def rotary_axes(q, k, position_ids, plan):
-    """``rotary_axes_forward`` with autograd."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+    """``rotary_axes_forward`` with reverse-mode autograd.  Forward-mode derivatives are refused (NotImplementedError);
+    ``torch.jit.trace`` records the call as one step."""
+    if torch.jit.is_tracing() or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
         return _RotaryAxes.apply(q, k, position_ids, plan)
     return rotary_axes_forward(q, k, position_ids, plan)

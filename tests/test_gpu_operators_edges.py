@@ -1,0 +1,43 @@
+"""GPU: LayerNorm, multi-axis rotary, gradient norm and 32-bit AdamW at the edges of what they promise."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def randn(dev, seed, *shape, scale=1.0, dtype=torch.float32):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).to(dev)
+
+
+# ------------------------------------------------------------------------------------------------ what torch cannot see
+@pytest.mark.parametrize("grad", [False, True])
+def test_traced_functions_follow_their_inputs(dev, grad):
+    from coat_amd.activation.norm import layer_norm
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes
+    plan, pos = RotaryAxes(32, (6, 10)), torch.arange(5, device=dev).expand(2, 1, 5)
+    w = randn(dev, 1, 32)
+
+    def f(x):
+        return layer_norm(rotary_axes(x, None, pos, plan)[0], w)
+
+    a, b = (randn(dev, s, 1, 5, 3, 32).requires_grad_(grad) for s in (2, 3))
+    traced = torch.jit.trace(f, (a,), check_trace=False)
+    for x in (b, a):
+        assert torch.equal(traced(x), f(x))
+
+
+def test_tangents_are_refused(dev):
+    import torch.autograd.forward_ad as fwAD
+
+    from coat_amd.activation.norm import layer_norm
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes
+    plan, pos = RotaryAxes(32, (6, 10)), torch.arange(5, device=dev).expand(2, 1, 5)
+    x = randn(dev, 2, 1, 5, 3, 32)
+    with fwAD.dual_level():
+        for grad in (False, True):
+            d = fwAD.make_dual(x.clone().requires_grad_(grad), torch.ones_like(x))
+            with pytest.raises(NotImplementedError):
+                layer_norm(d)
+            with pytest.raises(NotImplementedError):
+                rotary_axes(d, None, pos, plan)
+        assert torch.equal(layer_norm(x), layer_norm(x.clone()))

@@ -1,0 +1,88 @@
+"""CPU: calls of LayerNorm, multi-axis rotary, gradient norm and 32-bit AdamW at the edges of what they promise."""
+import pytest
+import torch
+
+HYPER = (0.9, 0.95, 1e-3, 0.1, 1e-8, 1)
+
+
+def binding_calls(x):
+    """Every entry of the binding that computes, on ``x`` [4, 8]; on the CPU each ends in a refusal."""
+    from coat_amd import _hip
+    native, stat, w = _hip.native(), torch.zeros(4), torch.zeros(8)
+    turns, axis = torch.zeros(4, dtype=torch.float64), torch.zeros(4, dtype=torch.int32)
+    return {"forward": lambda: native.layer_norm_forward(x, None, None, 1e-5),
+            "backward": lambda: native.layer_norm_backward(x, x, stat, stat, w, True, True, True),
+            "rotary": lambda: native.rotary_axes(x.view(1, 4, 1, 8), None, torch.zeros(1, 1, 4, dtype=torch.int64), turns, axis, 8, 1, 4, False, False),
+            "norm": lambda: native.grad_norm_multi([stat, x], 1.0),
+            "step": lambda: native.adamw_step_multi([stat, x], [stat, x], [stat, x], [stat, x], None, *HYPER, None)}
+
+
+# ------------------------------------------------------------------------------------------------ what torch cannot see
+@pytest.mark.parametrize("which", ["forward", "backward", "rotary", "norm", "step"])
+def test_forward_mode_tangents_are_refused_and_not_lost(which):
+    import torch.autograd.forward_ad as fwAD
+    x = torch.randn(4, 8)
+    with fwAD.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            binding_calls(fwAD.make_dual(x, torch.ones_like(x)))[which]()
+        with pytest.raises(RuntimeError, match="GPU"):  # a tensor without a tangent is none of this
+            binding_calls(x)[which]()
+
+
+def test_autograd_wrappers_refuse_tangents_with_and_without_requires_grad():
+    import torch.autograd.forward_ad as fwAD
+
+    from coat_amd.activation.norm import layer_norm
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes
+    plan, pos = RotaryAxes(8, (2, 2)), torch.zeros(2, 1, 4, dtype=torch.int64)
+    plan.tables = lambda device: (torch.zeros(4, dtype=torch.float64), torch.zeros(4, dtype=torch.int32))
+    x = torch.randn(1, 4, 1, 8)
+    with fwAD.dual_level():
+        with pytest.raises(NotImplementedError):
+            layer_norm(fwAD.make_dual(x, x))
+        with pytest.raises(NotImplementedError):
+            rotary_axes(fwAD.make_dual(x, x), None, pos, plan)
+
+
+@pytest.mark.parametrize("which", ["forward", "backward", "rotary", "norm", "step"])
+def test_recordings_of_operations_refuse_the_bare_calls(which):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn(4, 8)
+
+    def f(x):
+        binding_calls(x)[which]()
+        return x
+
+    with pytest.raises(NotImplementedError, match="trace"):
+        torch.jit.trace(f, (x,))
+    with pytest.raises(NotImplementedError, match="trace"):
+        make_fx(f)(x)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_a_trace_records_the_wrappers_as_one_step(grad, monkeypatch):
+    """The binding replaced by numpy on the CPU: what the traced function returns for other inputs."""
+    from coat_amd import _hip
+    from coat_amd.activation.norm import layer_norm
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes
+
+    class Native:
+        @staticmethod
+        def layer_norm_forward(x, w, b, eps):
+            y = torch.empty_like(x)
+            y.detach().numpy()[...] = x.detach().numpy() * 2
+            return y, torch.empty(x.shape[:-1]), torch.empty(x.shape[:-1])
+
+        @staticmethod
+        def rotary_axes(q, k, *rest):
+            out = torch.empty_like(q)
+            out.detach().numpy()[...] = q.detach().numpy() + 1
+            return out, None
+
+    monkeypatch.setattr(_hip, "native", lambda: Native)
+    plan, pos = RotaryAxes(8, (2, 2)), torch.zeros(2, 1, 4, dtype=torch.int64)
+    a, b = (torch.randn(1, 4, 1, 8).requires_grad_(grad) for _ in range(2))
+    with pytest.warns(torch.jit.TracerWarning):  # numpy in the stand-in
+        norm = torch.jit.trace(lambda x: layer_norm(x), (a,), check_trace=False)
+        turn = torch.jit.trace(lambda x: rotary_axes(x, None, pos, plan)[0], (a,), check_trace=False)
+    assert torch.equal(norm(b), b * 2) and torch.equal(turn(b), b + 1)
