@@ -16,7 +16,8 @@ class RotaryAxes:
     are passed through).  Pair j turns by ``position * theta ** -(j / P)``; with ``restart`` every section counts its own pairs,
     ``theta ** -(i / n)`` for pair i of a section of n.  Pair j is elements ``(j, j + P)`` of the head, the layout of the decoder
     layers; with ``pairs`` neighbours ``(2 j, 2 j + 1)``.  If CUDA is initialised, the tables are made on the device that is current
-    at construction; another device gets its own at the first use there (which must not be inside a graph capture)."""
+    at construction; another device gets its own at the first use there (which must not be inside a graph capture).  A copy, or a
+    plan that was saved and loaded, makes its own tables in the same way."""
 
     def __init__(self, head_dim, sections, theta=10000.0, restart=False, pairs=False):
         self.head_dim, self.sections, self.theta = int(head_dim), tuple(int(n) for n in sections), float(theta)
@@ -31,9 +32,20 @@ class RotaryAxes:
         self._axis = [a for a, n in enumerate(self.sections) for _ in range(n)]
         exponent = [i / n for n in self.sections for i in range(n)] if self.restart else [j / total for j in range(total)]
         self._freq = [self.theta ** -e for e in exponent]  # radians a position, in 64 bits
+        self._start_tables()
+
+    def _start_tables(self):
         self._tables = {}
         if torch.cuda.is_initialized():
             self.tables(torch.device("cuda", torch.cuda.current_device()))
+
+    def __getstate__(self):
+        """Without the tables: loading moves tensors between devices, but not the keys that say where they are."""
+        return {k: v for k, v in self.__dict__.items() if k != "_tables"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self._start_tables()
 
     def tables(self, device):
         """(turns a position fp64 [P], axis int32 [P]) on ``device``."""

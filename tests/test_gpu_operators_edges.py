@@ -41,3 +41,23 @@ def test_tangents_are_refused(dev):
             with pytest.raises(NotImplementedError):
                 rotary_axes(d, None, pos, plan)
         assert torch.equal(layer_norm(x), layer_norm(x.clone()))
+
+
+# ------------------------------------------------------------------------------------------------ rotary plans
+def test_loaded_and_copied_modules_rotate_as_before(dev):
+    import copy
+    import io
+
+    from coat_amd.models.coat_llama import CoatLlamaConfig, LlamaSdpaAttentionWithoutLinear
+    module = LlamaSdpaAttentionWithoutLinear(CoatLlamaConfig(hidden_size=256, num_attention_heads=2, rotary_sections=(16, 24, 24))).eval()
+    x = [randn(dev, s, 1, 20, 256, dtype=torch.bfloat16) for s in (1, 2, 3)]
+    pos = torch.randint(0, 50, (3, 1, 20), generator=torch.Generator().manual_seed(4)).to(dev)
+    want = module(*x, position_ids=pos)[0]
+    for where in ("cpu", dev):
+        buffer = io.BytesIO()
+        torch.save(module, buffer)
+        buffer.seek(0)
+        loaded = torch.load(buffer, map_location=where, weights_only=False)
+        for other in (loaded, copy.deepcopy(loaded)):
+            assert all(t.device == d for d, pair in other.rotary_axes._tables.items() for t in pair)
+            assert torch.equal(other(*x, position_ids=pos)[0], want)

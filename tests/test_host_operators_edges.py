@@ -86,3 +86,25 @@ def test_a_trace_records_the_wrappers_as_one_step(grad, monkeypatch):
         norm = torch.jit.trace(lambda x: layer_norm(x), (a,), check_trace=False)
         turn = torch.jit.trace(lambda x: rotary_axes(x, None, pos, plan)[0], (a,), check_trace=False)
     assert torch.equal(norm(b), b * 2) and torch.equal(turn(b), b + 1)
+
+
+# ------------------------------------------------------------------------------------------------ rotary plans
+def test_plans_are_saved_and_copied_without_their_tables():
+    """Tables of another device under the key of the first one would be read as that device's memory."""
+    import copy
+    import io
+
+    from coat_amd.models.rotary import RotaryAxes
+    plan, there = RotaryAxes(32, (6, 10), theta=500.0, restart=True, pairs=True), torch.device("cuda", 0)
+    old = {**plan.__dict__, "_tables": {there: (torch.zeros(16, dtype=torch.float64), torch.zeros(16, dtype=torch.int32))}}
+    plan._tables.update(old["_tables"])
+    buffer = io.BytesIO()
+    torch.save(plan, buffer)
+    buffer.seek(0)
+    loaded, before = torch.load(buffer, map_location="cpu", weights_only=False), RotaryAxes.__new__(RotaryAxes)
+    before.__setstate__(old)  # a file that still holds tables
+    for other in (loaded, before, copy.copy(plan), copy.deepcopy(plan)):
+        assert there not in other._tables or other._tables[there][0].device == there
+        assert {k: v for k, v in other.__dict__.items() if k != "_tables"} == {k: v for k, v in plan.__dict__.items() if k != "_tables"}
+        turns, axis = other.tables(torch.device("cpu"))
+        assert turns.tolist() == plan.tables(torch.device("cpu"))[0].tolist() and axis.tolist() == [0] * 6 + [1] * 10
