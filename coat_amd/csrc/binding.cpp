@@ -251,6 +251,9 @@ PyObject* rotary_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t D = whole(a[5]), axes = whole(a[6]), pairs = whole(a[7]);
     TORCH_CHECK_VALUE(q || k, who, ": neither q nor k given");
     unrecorded(who, {q, k});
+    TORCH_CHECK_VALUE(turns.scalar_type() == at::kDouble && turns.numel() == pairs && turns.is_contiguous() && axis.scalar_type() == at::kInt &&
+                          axis.numel() == pairs && axis.is_contiguous(),
+                      who, ": the plan's tables must be contiguous, fp64 and int32, with one element for each of ", pairs, " pairs");
     const at::Tensor& first = q ? *q : *k;
     on_gpu(first);
     for (const at::Tensor* t : {q, k}) {
@@ -259,6 +262,8 @@ PyObject* rotary_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
                           ": expected [batch, seq, heads, ", D, "] tensors of one batch, got ", t->sizes());
         TORCH_CHECK_VALUE(t->scalar_type() == first.scalar_type() && t->device() == first.device(), who, ": q and k must have one dtype and device");
     }
+    TORCH_CHECK_VALUE(turns.device() == first.device() && axis.device() == first.device(), who, ": the plan's tables are on ", turns.device(),
+                      " and ", axis.device(), ", q and k on ", first.device());
     const int dt = code_of(first.scalar_type());
     const int64_t B = first.size(0), S = first.size(1);
     TORCH_CHECK_VALUE(pos.dim() == 3 && pos.size(0) == axes, who, ": expected position_ids of shape [", axes, ", batch, seq], got ", pos.sizes());

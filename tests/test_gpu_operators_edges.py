@@ -61,3 +61,13 @@ def test_loaded_and_copied_modules_rotate_as_before(dev):
         for other in (loaded, copy.deepcopy(loaded)):
             assert all(t.device == d for d, pair in other.rotary_axes._tables.items() for t in pair)
             assert torch.equal(other(*x, position_ids=pos)[0], want)
+
+
+def test_tables_of_another_device_are_refused(dev):
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes_forward
+    plan, q, pos = RotaryAxes(32, (6, 10)), randn(dev, 1, 1, 5, 2, 32), torch.arange(5, device=dev).expand(2, 1, 5)
+    turns, axis = plan.tables(q.device)
+    for bad in ((turns.cpu(), axis), (turns, axis.cpu())):
+        plan._tables[q.device] = bad
+        with pytest.raises(ValueError, match="tables"):
+            rotary_axes_forward(q, None, pos, plan)

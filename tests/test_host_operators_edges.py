@@ -108,3 +108,13 @@ def test_plans_are_saved_and_copied_without_their_tables():
         assert {k: v for k, v in other.__dict__.items() if k != "_tables"} == {k: v for k, v in plan.__dict__.items() if k != "_tables"}
         turns, axis = other.tables(torch.device("cpu"))
         assert turns.tolist() == plan.tables(torch.device("cpu"))[0].tolist() and axis.tolist() == [0] * 6 + [1] * 10
+
+
+def test_tables_that_are_not_a_plans_are_refused():
+    from coat_amd import _hip
+    q, pos = torch.zeros(1, 3, 2, 8), torch.zeros(2, 1, 3, dtype=torch.int64)
+    turns, axis = torch.zeros(4, dtype=torch.float64), torch.zeros(4, dtype=torch.int32)
+    for bad in ((turns.float(), axis), (turns, axis.long()), (turns[:3], axis), (turns, axis[:3]), (torch.zeros(8, dtype=torch.float64)[::2], axis),
+                (turns, torch.zeros(8, dtype=torch.int32)[::2])):
+        with pytest.raises(ValueError, match="tables"):
+            _hip.native().rotary_axes(q, None, pos, *bad, 8, 2, 4, False, False)
