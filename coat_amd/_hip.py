@@ -91,6 +91,9 @@ SIGNATURES = {
 _lib = None
 _native = None
 
+# device index -> handle of torch's current stream there, without a stream object where torch has that
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
 
 def native():
     """The compiled binding (coat_amd/_binding.so) of the operators whose small calls are bound by the host, holding this library's
@@ -108,8 +111,7 @@ def native():
                                "with `python -m coat_amd.build`")
         names = ("coat_status_string", "coat_layer_norm_forward", "coat_layer_norm_partials", "coat_layer_norm_backward", "coat_rope_axes",
                  "coat_grad_norm_partials", "coat_grad_norm_multi", "coat_adamw_step_multi")
-        stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
-        _binding.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names}, stream_of)
+        _binding.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in names}, raw_stream)
         _native = _binding
     return _native
 

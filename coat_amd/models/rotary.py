@@ -17,7 +17,8 @@ class RotaryAxes:
     ``theta ** -(i / n)`` for pair i of a section of n.  Pair j is elements ``(j, j + P)`` of the head, the layout of the decoder
     layers; with ``pairs`` neighbours ``(2 j, 2 j + 1)``.  If CUDA is initialised, the tables are made on the device that is current
     at construction; another device gets its own at the first use there (which must not be inside a graph capture).  A copy, or a
-    plan that was saved and loaded, makes its own tables in the same way."""
+    plan that was saved and loaded, makes its own tables in the same way.  A plan may be dropped while work that uses it is still
+    queued, on any stream; a captured graph reads its tables at every replay and needs the plan alive."""
 
     def __init__(self, head_dim, sections, theta=10000.0, restart=False, pairs=False):
         self.head_dim, self.sections, self.theta = int(head_dim), tuple(int(n) for n in sections), float(theta)
@@ -35,13 +36,13 @@ class RotaryAxes:
         self._start_tables()
 
     def _start_tables(self):
-        self._tables = {}
+        self._tables, self._home = {}, {}  # by device: the tables, and the stream whose order their memory follows
         if torch.cuda.is_initialized():
             self.tables(torch.device("cuda", torch.cuda.current_device()))
 
     def __getstate__(self):
         """Without the tables: loading moves tensors between devices, but not the keys that say where they are."""
-        return {k: v for k, v in self.__dict__.items() if k != "_tables"}
+        return {k: v for k, v in self.__dict__.items() if k not in ("_tables", "_home")}
 
     def __setstate__(self, state):
         self.__dict__.update(state)
@@ -52,7 +53,16 @@ class RotaryAxes:
         if device not in self._tables:
             turns = torch.tensor([f / (2.0 * math.pi) for f in self._freq], dtype=torch.float64, device=device)
             self._tables[device] = turns, torch.tensor(self._axis, dtype=torch.int32, device=device)
+            self._home[device] = _hip.raw_stream(device.index) if device.type == "cuda" else None
         return self._tables[device]
+
+    def _use(self, device):
+        """``tables``, kept from reuse until what is queued on the current stream has read them: the caller cannot see these tensors."""
+        tables = self.tables(device)
+        if device.type == "cuda" and _hip.raw_stream(device.index) != self._home[device]:
+            for t in tables:
+                t.record_stream(torch.cuda.current_stream(device))
+        return tables
 
     def cos_sin(self, position_ids, dtype):
         """cos / sin [B, S, head_dim] from torch operations on any device, for heads that turn whole in the (j, j + P) layout;
@@ -71,7 +81,7 @@ def _rotate(q, k, position_ids, plan, inverse):
     first = k if q is None else q
     if first is None:
         raise ValueError("rotary_axes: neither q nor k given")
-    turns, axis = plan.tables(first.device)
+    turns, axis = plan._use(first.device)
     return _hip.native().rotary_axes(q, k, position_ids, turns, axis, plan.head_dim, len(plan.sections), plan.turning, plan.pairs, inverse)
 
 

@@ -71,3 +71,23 @@ def test_tables_of_another_device_are_refused(dev):
         plan._tables[q.device] = bad
         with pytest.raises(ValueError, match="tables"):
             rotary_axes_forward(q, None, pos, plan)
+
+
+def test_a_plan_may_be_dropped_while_another_stream_still_reads_its_tables(dev):
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes, rotary_axes_forward
+    q, pos = randn(dev, 1, 1, 50, 4, 128).requires_grad_(), torch.arange(50, device=dev).expand(3, 1, 50)
+    want = rotary_axes_forward(q, None, pos, RotaryAxes(128, (16, 24, 24)))[0]
+    work, side = randn(dev, 2, 4096, 4096), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    plan = RotaryAxes(128, (16, 24, 24))
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            work = (work @ work).clamp_(-1, 1)  # the rotation waits behind this
+        out = rotary_axes(q, None, pos, plan)[0]
+        out.backward(want.detach(), retain_graph=False)
+    del plan
+    other = [torch.full((64,), 7.5, dtype=torch.float64, device=dev) for _ in range(200)] + [torch.full((64,), 1, dtype=torch.int32, device=dev) for _ in range(200)]
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and len(other) == 400
+    assert torch.allclose(q.grad, q, rtol=1e-5, atol=1e-5)  # turned there and back

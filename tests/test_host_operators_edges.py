@@ -105,7 +105,7 @@ def test_plans_are_saved_and_copied_without_their_tables():
     before.__setstate__(old)  # a file that still holds tables
     for other in (loaded, before, copy.copy(plan), copy.deepcopy(plan)):
         assert there not in other._tables or other._tables[there][0].device == there
-        assert {k: v for k, v in other.__dict__.items() if k != "_tables"} == {k: v for k, v in plan.__dict__.items() if k != "_tables"}
+        assert {k: v for k, v in other.__dict__.items() if k not in ("_tables", "_home")} == {k: v for k, v in plan.__dict__.items() if k not in ("_tables", "_home")}
         turns, axis = other.tables(torch.device("cpu"))
         assert turns.tolist() == plan.tables(torch.device("cpu"))[0].tolist() and axis.tolist() == [0] * 6 + [1] * 10
 
@@ -118,3 +118,29 @@ def test_tables_that_are_not_a_plans_are_refused():
                 (turns, torch.zeros(8, dtype=torch.int32)[::2])):
         with pytest.raises(ValueError, match="tables"):
             _hip.native().rotary_axes(q, None, pos, *bad, 8, 2, 4, False, False)
+
+
+def test_tables_used_on_another_stream_than_their_own_are_recorded_there(monkeypatch):
+    """The caller of a plan cannot do that: the memory of a dropped plan would be reused under a kernel that still reads it."""
+    from coat_amd import _hip
+    from coat_amd.models.rotary import RotaryAxes
+
+    class Table:
+        def __init__(self):
+            self.recorded = []
+
+        def record_stream(self, s):
+            self.recorded.append(s)
+
+    current, there = [7], torch.device("cuda", 0)
+    monkeypatch.setattr(_hip, "raw_stream", lambda index: current[0])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: (device, current[0]))
+    plan = RotaryAxes(32, (6, 10))
+    made = []
+    monkeypatch.setattr(torch, "tensor", lambda *a, **kw: made.append(Table()) or made[-1])
+    assert plan._use(there) == tuple(made) and not any(t.recorded for t in made)
+    current[0] = 9
+    plan._use(there)
+    current[0] = 7
+    plan._use(there)
+    assert [t.recorded for t in made] == [[(there, 9)], [(there, 9)]]
