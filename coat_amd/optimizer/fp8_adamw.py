@@ -50,8 +50,9 @@ class CoatAdamW(Optimizer):
         16-bit parameters (state key ``master``), made at the first step: what is written into the parameters from outside after
         that is lost at the next one.  Both may be given per parameter group.  ``max_grad_norm``: the gradients of all groups, on
         one device, are clipped to that global 2-norm of this process's gradients inside the step (``grad_norm`` then holds the
-        norm of the last step, on the device; the gradients themselves stay as they are).  None of the three is in the
-        reference."""
+        norm of the last step, on the device; the gradients themselves stay as they are).  It is kept in the parameter groups,
+        where it may be changed between steps and where ``load_state_dict`` restores it, and is the same in all of them: ``step``
+        raises otherwise.  None of the three is in the reference."""
         # multi_tensor (not in the reference): parameters of one dtype, device and step count share kernel launches
         self.multi_tensor = multi_tensor
         self.qargs = QuantizationConfig() if qargs is None else qargs
@@ -87,9 +88,11 @@ class CoatAdamW(Optimizer):
             raise ValueError(f"Invalid state_bits: {bits} (8 or 32)")
         if param_group.get("master_weights", self.defaults.get("master_weights", False)) and bits != 32:
             raise ValueError("master_weights needs state_bits=32")
-        clip = self.defaults.get("max_grad_norm")
+        clip = (self.param_groups[0] if self.param_groups else self.defaults).get("max_grad_norm")
         if param_group.get("max_grad_norm", clip) != clip:
             raise ValueError("max_grad_norm is one for all parameter groups")
+        if clip is not None or "max_grad_norm" in self.defaults:
+            param_group["max_grad_norm"] = clip  # that of the groups there, which may have changed since construction
         super().add_param_group(param_group)
 
     # ------------------------------------------------------------------ state
@@ -179,7 +182,9 @@ class CoatAdamW(Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        max_grad_norm, scale = self.defaults.get("max_grad_norm"), None
+        max_grad_norm, scale = (self.param_groups[0].get("max_grad_norm") if self.param_groups else None), None
+        if any(group.get("max_grad_norm") != max_grad_norm for group in self.param_groups):
+            raise ValueError("max_grad_norm is one for all parameter groups")
         if max_grad_norm is not None:
             grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
             if any(g.is_sparse for g in grads):

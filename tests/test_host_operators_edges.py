@@ -144,3 +144,56 @@ def test_tables_used_on_another_stream_than_their_own_are_recorded_there(monkeyp
     current[0] = 7
     plan._use(there)
     assert [t.recorded for t in made] == [[(there, 9)], [(there, 9)]]
+
+
+# ------------------------------------------------------------------------------------------------ CoatAdamW
+class Calls:
+    """The kernels' Python entries replaced: what the optimizer hands them."""
+
+    def __init__(self, monkeypatch):
+        from coat_amd.optimizer import qoptim_cuda
+        self.clip, self.steps = [], []
+        monkeypatch.setattr(qoptim_cuda, "grad_norm_multi", lambda grads, most: self.clip.append(most) or (torch.tensor(2.0), torch.tensor(0.25)))
+        for name in ("adamw_step_multi", "fp8_adamw_expand_step_multi", "fp8_adamw_step_multi", "fp8_adamw_expand_step", "fp8_adamw_step"):
+            monkeypatch.setattr(qoptim_cuda, name, lambda *a, _name=name, **kw: self.steps.append((_name, a, kw)))
+
+
+def parameter(n=4):
+    p = torch.nn.Parameter(torch.zeros(n))
+    p.grad = torch.ones(n)
+    return p
+
+
+def test_clipping_follows_the_parameter_groups(monkeypatch):
+    from coat_amd.optimizer.fp8_adamw import CoatAdamW
+    calls = Calls(monkeypatch)
+    first = CoatAdamW([parameter()], state_bits=32, max_grad_norm=0.5)
+    first.step()
+    assert calls.clip == [0.5] and first.grad_norm == 2.0
+    for kw in (dict(), dict(state_bits=32), dict(max_grad_norm=3.0)):
+        resumed = CoatAdamW([parameter()], **kw)
+        resumed.load_state_dict(first.state_dict())
+        assert resumed.param_groups[0]["max_grad_norm"] == 0.5
+        resumed.step()
+        assert calls.clip.pop() == 0.5 and calls.steps[-1][2]["grad_scale"] == 0.25
+    first.param_groups[0]["max_grad_norm"] = 0.01
+    first.step()
+    assert calls.clip[-1] == 0.01
+    first.add_param_group(dict(params=[parameter()]))  # joins the others
+    assert first.param_groups[1]["max_grad_norm"] == 0.01
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        first.add_param_group(dict(params=[parameter()], max_grad_norm=0.5))
+    first.step()
+    for group in first.param_groups:
+        group["max_grad_norm"] = None
+    n = len(calls.clip)
+    first.step()
+    assert len(calls.clip) == n and calls.steps[-1][2]["grad_scale"] is None
+    first.add_param_group(dict(params=[parameter()]))
+    first.step()
+    assert len(calls.clip) == n
+    first.param_groups[1]["max_grad_norm"] = 1.0
+    steps, counts = len(calls.steps), [int(s["step"]) for s in first.state.values()]
+    with pytest.raises(ValueError, match="max_grad_norm"):
+        first.step()
+    assert len(calls.steps) == steps and [int(s["step"]) for s in first.state.values()] == counts  # before anything is stepped
