@@ -136,7 +136,8 @@ class CoatAdamW(Optimizer):
         """torch's Optimizer.load_state_dict casts every floating-point state tensor to the parameter dtype;
         FP8 codes and fp32 group vectors must keep theirs, so the mapping is redone here with that policy
         (reference :158-262): ``step`` is left alone, every other tensor must be e4m3 / e5m2 / fp32 and is
-        only moved to the parameter's device."""
+        only moved to the parameter's device.  Groups that say nothing of ``state_bits``, ``master_weights`` or ``max_grad_norm``
+        (plain 8-bit ones, those of another optimizer) keep this optimizer's; moments that do not fit ``state_bits=32`` are refused."""
         state_dict = state_dict.copy()
         for pre_hook in self._optimizer_load_state_dict_pre_hooks.values():
             replaced = pre_hook(self, state_dict)
@@ -148,6 +149,15 @@ class CoatAdamW(Optimizer):
             raise ValueError("loaded state dict has a different number of parameter groups")
         if any(len(g["params"]) != len(s["params"]) for g, s in zip(groups, saved_groups)):
             raise ValueError("loaded state dict contains a parameter group that doesn't match the size of optimizer's group")
+        for g, s in zip(groups, saved_groups):
+            s.update({k: g[k] for k in ("state_bits", "master_weights", "max_grad_norm") if k in g and k not in s})
+            bits = s.get("state_bits", 8)
+            if s.get("master_weights", False) and bits != 32:
+                raise ValueError("master_weights needs state_bits=32")
+            for key in s["params"] if bits == 32 else ():
+                held = [t.dtype for name, t in state_dict["state"].get(key, {}).items() if name in ("exp_avg", "exp_avg_sq")]
+                if any(dtype != torch.float32 for dtype in held):
+                    raise ValueError(f"loaded moments are {held[0]}, but the parameter group has state_bits=32")
         id_map = dict(zip(chain.from_iterable(s["params"] for s in saved_groups),
                           chain.from_iterable(g["params"] for g in groups)))
 

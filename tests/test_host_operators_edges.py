@@ -197,3 +197,44 @@ def test_clipping_follows_the_parameter_groups(monkeypatch):
     with pytest.raises(ValueError, match="max_grad_norm"):
         first.step()
     assert len(calls.steps) == steps and [int(s["step"]) for s in first.state.values()] == counts  # before anything is stepped
+
+
+def test_states_that_say_nothing_of_bits_masters_and_clipping_keep_the_optimizers(monkeypatch):
+    from coat_amd.optimizer.fp8_adamw import CoatAdamW
+    calls, mine = Calls(monkeypatch), dict(state_bits=32, master_weights=True, max_grad_norm=0.5)
+    half = torch.nn.Parameter(torch.zeros(4, dtype=torch.bfloat16))
+    opt = CoatAdamW([half], **mine)
+    opt.load_state_dict(CoatAdamW([parameter()]).state_dict())  # nothing stepped yet: no moments that could not fit
+    assert all(opt.param_groups[0][k] == v for k, v in mine.items())
+    half.grad = torch.ones_like(half)
+    opt.step()
+    name, args, kw = calls.steps[-1]
+    assert name == "adamw_step_multi" and kw["masters"][0].dtype == torch.float32 and calls.clip == [0.5]
+    p = parameter()
+    other = torch.optim.AdamW([p], lr=0.02)
+    other.step()
+    opt = CoatAdamW([p], **mine)
+    opt.load_state_dict(other.state_dict())  # fp32 moments of torch's AdamW
+    assert opt.param_groups[0]["lr"] == 0.02 and opt.param_groups[0]["state_bits"] == 32
+    opt.step()
+    assert calls.steps[-1][0] == "adamw_step_multi" and calls.steps[-1][1][2][0] is opt.state[p]["exp_avg"] and int(opt.state[p]["step"]) == 2
+    eight = CoatAdamW([parameter()])
+    eight.step()
+    opt = CoatAdamW([parameter()], state_bits=32)
+    with pytest.raises(ValueError, match="state_bits=32"):
+        opt.load_state_dict(eight.state_dict())
+    assert not opt.state and opt.param_groups[0]["state_bits"] == 32  # nothing taken over
+    opt = CoatAdamW([dict(params=[parameter()], state_bits=8)], state_bits=32)  # a group of its own
+    opt.load_state_dict(eight.state_dict())
+    opt.step()
+    assert opt.param_groups[0]["state_bits"] == 8 and calls.steps[-1][0] in ("fp8_adamw_expand_step", "fp8_adamw_step")
+    opt = CoatAdamW([parameter()], state_bits=32, master_weights=True)
+    with pytest.raises(ValueError, match="master_weights"):
+        opt.load_state_dict(CoatAdamW([dict(params=[parameter()], state_bits=8)], state_bits=32).state_dict())
+    restored = CoatAdamW([parameter()])  # and what the state does say is restored, as before
+    wide = CoatAdamW([parameter()], state_bits=32)
+    wide.step()
+    restored.load_state_dict(wide.state_dict())
+    assert restored.param_groups[0]["state_bits"] == 32
+    restored.step()
+    assert calls.steps[-1][0] == "adamw_step_multi"
