@@ -50,7 +50,8 @@ class CoatAdamW(Optimizer):
         16-bit parameters (state key ``master``), made at the first step: what is written into the parameters from outside after
         that is lost at the next one.  Both may be given per parameter group.  ``max_grad_norm``: the gradients of all groups, on
         one device, are clipped to that global 2-norm of this process's gradients inside the step (``grad_norm`` then holds the
-        norm of the last step, on the device; the gradients themselves stay as they are).  It is kept in the parameter groups,
+        norm of the last step, on the device, or None after a step without clipping or without gradients; the gradients themselves
+        stay as they are).  It is kept in the parameter groups,
         where it may be changed between steps and where ``load_state_dict`` restores it, and is the same in all of them: ``step``
         raises otherwise.  None of the three is in the reference."""
         # multi_tensor (not in the reference): parameters of one dtype, device and step count share kernel launches
@@ -195,6 +196,7 @@ class CoatAdamW(Optimizer):
         max_grad_norm, scale = (self.param_groups[0].get("max_grad_norm") if self.param_groups else None), None
         if any(group.get("max_grad_norm") != max_grad_norm for group in self.param_groups):
             raise ValueError("max_grad_norm is one for all parameter groups")
+        self.grad_norm = None
         if max_grad_norm is not None:
             grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
             if any(g.is_sparse for g in grads):

@@ -238,3 +238,15 @@ def test_states_that_say_nothing_of_bits_masters_and_clipping_keep_the_optimizer
     assert restored.param_groups[0]["state_bits"] == 32
     restored.step()
     assert calls.steps[-1][0] == "adamw_step_multi"
+
+
+def test_the_norm_is_that_of_the_last_step(monkeypatch):
+    from coat_amd.optimizer.fp8_adamw import CoatAdamW
+    Calls(monkeypatch)
+    p = parameter()
+    opt = CoatAdamW([p], state_bits=32, max_grad_norm=0.5)
+    opt.step()
+    assert opt.grad_norm == 2.0
+    p.grad = None
+    opt.step()
+    assert opt.grad_norm is None
