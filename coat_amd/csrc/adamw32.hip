@@ -16,6 +16,7 @@
 
 #include "coat_host.h"
 #include "elem_io.h"
+#include "tensor_list.h"
 
 namespace coat {
 
@@ -130,6 +131,8 @@ __global__ __launch_bounds__(1024) void k_grad_norm(const double* __restrict__ p
 // ------------------------------------------------------------------------------------------------ the step
 constexpr int kStepMax = 76;        // tensors per launch: what the 4 KB of kernel arguments hold
 constexpr int kStepChunk = 1024;    // elements a block steps
+constexpr int64_t kStepBlocks = coat_max_blocks(256);  // per launch
+constexpr int64_t kNormChunks = 0x7fffffff;            // per launch: their numbers are 32-bit
 struct Step32Tensor {
     void* p;
     const void* g;
@@ -187,29 +190,6 @@ static bool opt_dtype(int dt) { return dt == COAT_F32 || dt == COAT_BF16 || dt =
 static bool elem_aligned(const void* p, int dt) { return ((uintptr_t)p & (dt == COAT_F32 ? 3u : 1u)) == 0; }
 static int64_t norm_chunks(int64_t numel) { return (numel + kNormChunk - 1) / kNormChunk; }
 
-// Calls fn(first, last, chunks) for each run of tensors that one launch takes: at most `most` tensors that are not empty and
-// fewer than 2^31 chunks.  Returns COAT_ESHAPE if one tensor alone has more.
-template <typename F> static int for_each_launch(int count, const int64_t* numel, int64_t chunk, int most, F fn) {
-    for (int i = 0; i < count;) {
-        const int first = i;
-        int used = 0;
-        int64_t chunks = 0;
-        for (; i < count && used < most; i++) {
-            if (numel[i] == 0) continue;
-            const int64_t c = (numel[i] + chunk - 1) / chunk;
-            if (chunks + c > 0x7fffffffll) {
-                if (used == 0) return COAT_ESHAPE;
-                break;
-            }
-            chunks += c;
-            used++;
-        }
-        if (used == 0) break;  // only empty tensors were left
-        if (const int rc = fn(first, i, chunks)) return rc;
-    }
-    return COAT_OK;
-}
-
 // Whether a tensor that is written shares memory with another tensor of a launch (a block would then read what another has
 // stepped already).  `spans`: begin, end and whether it is written; sorted here.
 struct Span {
@@ -232,7 +212,7 @@ extern "C" int coat_grad_norm_partials(int count, const int64_t* numel) {
     int64_t total = 0;
     for (int i = 0; i < count; i++)
         if (numel[i] < 0) return COAT_EINVAL;
-    const int rc = for_each_launch(count, numel, kNormChunk, kNormMax, [&](int, int, int64_t chunks) {
+    const int rc = coat_for_each_launch(count, numel, kNormChunk, kNormMax, kNormChunks, [&](int, int, int64_t chunks) {
         total += chunks < kNormBlocks ? chunks : kNormBlocks;
         return total > 0x7fffffff ? COAT_ESHAPE : COAT_OK;
     });
@@ -254,7 +234,7 @@ extern "C" int coat_grad_norm_multi(int count, const void* const* grads, const i
     }
     hipStream_t st = (hipStream_t)stream;
     double* at = partial;
-    const int rc = for_each_launch(count, numel, kNormChunk, kNormMax, [&](int first, int last, int64_t chunks) {
+    const int rc = coat_for_each_launch(count, numel, kNormChunk, kNormMax, kNormChunks, [&](int first, int last, int64_t chunks) {
         NormArgs A;
         A.count = 0;
         uint32_t c = 0;
@@ -288,14 +268,14 @@ extern "C" int coat_adamw_step_multi(int count, void* const* params, int p_dtype
     if (!elem_aligned(grad_scale, COAT_F32)) return COAT_EALIGN;
     for (int i = 0; i < count; i++) {  // everything is checked before the first launch
         if (numel[i] < 0) return COAT_EINVAL;
-        if (numel[i] > ((int64_t)0x7fffffff) * kStepChunk) return COAT_ESHAPE;
+        if (numel[i] > kStepBlocks * kStepChunk) return COAT_ESHAPE;
         if (numel[i] == 0) continue;
         if (!params[i] || !grads[i] || !exp_avg[i] || !exp_avg_sq[i] || (masters && !masters[i])) return COAT_EINVAL;
         if (!elem_aligned(params[i], p_dtype) || !elem_aligned(grads[i], g_dtype) || !elem_aligned(exp_avg[i], COAT_F32) ||
             !elem_aligned(exp_avg_sq[i], COAT_F32) || (masters && !elem_aligned(masters[i], COAT_F32)))
             return COAT_EALIGN;
     }
-    const int checked = for_each_launch(count, numel, kStepChunk, kStepMax, [&](int first, int last, int64_t) {
+    const int checked = coat_for_each_launch(count, numel, kStepChunk, kStepMax, kStepBlocks, [&](int first, int last, int64_t) {
         Span spans[5 * kStepMax];
         int n = 0;
         for (int i = first; i < last; i++) {
@@ -324,7 +304,7 @@ extern "C" int coat_adamw_step_multi(int count, void* const* params, int p_dtype
     H.c1 = (float)(1.0 - pow(beta1, (double)step));
     H.inv_c2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
     hipStream_t st = (hipStream_t)stream;
-    return for_each_launch(count, numel, kStepChunk, kStepMax, [&](int first, int last, int64_t chunks) {
+    return coat_for_each_launch(count, numel, kStepChunk, kStepMax, kStepBlocks, [&](int first, int last, int64_t chunks) {
         Step32Args A;
         A.count = 0;
         A.grad_scale = grad_scale;

@@ -1,0 +1,32 @@
+// Lists of tensors on the host, ahead of launches that take several of them: no device code, nothing of HIP.
+#pragma once
+#include <stdint.h>
+
+#include "../../include/coat_hip.h"
+
+// Blocks of `threads` that a launch takes in one dimension: HIP has fewer than 2^32 threads there.
+constexpr int64_t coat_max_blocks(int threads) { return 0xffffffffll / threads; }
+
+// Calls fn(first, last, chunks) for each run of tensors that one launch takes: at most `most` tensors that are not empty and
+// `most_chunks` chunks of `chunk` elements.  Returns COAT_ESHAPE if one tensor alone has more.
+template <typename F>
+static int coat_for_each_launch(int count, const int64_t* numel, int64_t chunk, int most, int64_t most_chunks, F fn) {
+    for (int i = 0; i < count;) {
+        const int first = i;
+        int used = 0;
+        int64_t chunks = 0;
+        for (; i < count && used < most; i++) {
+            if (numel[i] == 0) continue;
+            const int64_t c = (numel[i] + chunk - 1) / chunk;
+            if (chunks + c > most_chunks) {
+                if (used == 0) return COAT_ESHAPE;
+                break;
+            }
+            chunks += c;
+            used++;
+        }
+        if (used == 0) break;  // only empty tensors were left
+        if (const int rc = fn(first, i, chunks)) return rc;
+    }
+    return COAT_OK;
+}

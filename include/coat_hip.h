@@ -429,7 +429,8 @@ int coat_grad_norm_partials(int count, const int64_t* numel);
 int coat_grad_norm_multi(int count, const void* const* grads, const int* dtypes, const int64_t* numel, float max_norm,
                          double* partial, int n_partial, float* out, void* stream);
 
-/* AdamW step of several tensors with both moments in fp32, 76 tensors to a launch; the formula of coat_fp8_adamw_step_multi.
+/* AdamW step of several tensors with both moments in fp32, at most 76 tensors and (2^24 - 1) * 1024 elements to a launch (a single
+ * tensor with more is COAT_ESHAPE); the formula of coat_fp8_adamw_step_multi.
  * params of p_dtype; grads of p_dtype or fp32; masters NULL, or fp32 copies of 16-bit parameters that are stepped instead, the
  * parameter receiving their rounding.  hyper: host array of five doubles: beta1, beta2 (both in [0, 1)), lr, weight decay,
  * eps.  grad_scale: NULL, or one fp32 in device memory that the gradients are multiplied by (out[1] above).  Host arrays are

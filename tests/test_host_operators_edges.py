@@ -250,3 +250,63 @@ def test_the_norm_is_that_of_the_last_step(monkeypatch):
     p.grad = None
     opt.step()
     assert opt.grad_norm is None
+
+
+# ------------------------------------------------------------------------------------------------ sizes of launches
+STEP_BLOCKS, STEP_CHUNK, STEP_TENSORS = (2 ** 32 - 1) // 256, 1024, 76
+
+
+@pytest.fixture(scope="module")
+def runs(tmp_path_factory):
+    """The library's own split of a list into launches, compiled for the host alone: [(first, last, chunks)] and the status."""
+    import ctypes
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "coat_amd", "csrc")
+    where = tmp_path_factory.mktemp("runs")
+    (where / "runs.cpp").write_text(f'#include "{csrc}/tensor_list.h"\n' + """
+extern "C" int64_t max_blocks(int threads) { return coat_max_blocks(threads); }
+extern "C" int runs(int count, const int64_t* numel, int64_t chunk, int most, int64_t most_chunks, int64_t* out, int* n) {
+    *n = 0;
+    return coat_for_each_launch(count, numel, chunk, most, most_chunks, [&](int first, int last, int64_t chunks) {
+        int64_t* o = out + 3 * (*n)++;
+        o[0] = first, o[1] = last, o[2] = chunks;
+        return COAT_OK;
+    });
+}""")
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-o", str(where / "runs.so"), str(where / "runs.cpp")], check=True)
+    lib = ctypes.CDLL(str(where / "runs.so"))
+    lib.max_blocks.restype = ctypes.c_int64
+
+    def f(numel, chunk=STEP_CHUNK, most=STEP_TENSORS, most_chunks=STEP_BLOCKS):
+        assert lib.max_blocks(256) == STEP_BLOCKS
+        out, n = (ctypes.c_int64 * (3 * len(numel) + 3))(), ctypes.c_int()
+        status = lib.runs(len(numel), (ctypes.c_int64 * len(numel))(*numel), ctypes.c_int64(chunk), most, ctypes.c_int64(most_chunks), out, ctypes.byref(n))
+        return status, [tuple(out[3 * i:3 * i + 3]) for i in range(n.value)]
+
+    return f
+
+
+def test_lists_are_split_into_launches_that_can_start(runs):
+    """HIP takes fewer than 2^32 threads: 2^24 - 1 blocks of 256."""
+    for numel in ([2 ** 33] * 5, [2 ** 34 - 1024, 1024, 2 ** 34 - 1024], [1, 2 ** 34 - 1024, 0, 1, 0], [5] * 200, [0] * 10, [], [2 ** 28 + 1] * 150,
+                  [0, 0, 2 ** 34 - 2048, 1, 1024, 0]):
+        status, launches = runs(numel)
+        assert status == 0
+        covered = [i for first, last, _ in launches for i in range(first, last) if numel[i]]
+        assert covered == [i for i, n in enumerate(numel) if n]  # each tensor once, in order
+        for first, last, chunks in launches:
+            assert chunks == sum(-(-n // STEP_CHUNK) for n in numel[first:last]) and chunks * 256 < 2 ** 32
+            assert 1 <= sum(n > 0 for n in numel[first:last]) <= STEP_TENSORS
+    assert runs([2 ** 34 - 1023])[0] == runs([4, 2 ** 34])[0] == -2  # COAT_ESHAPE
+
+
+def test_steps_of_tensors_that_no_launch_takes_are_refused_before_the_first():
+    import ctypes
+
+    from coat_amd import _hip
+    L, p = _hip.lib(), 1 << 12
+    vp, hyper = ctypes.c_void_p * 2, (ctypes.c_double * 5)(0.9, 0.95, 1e-3, 0.1, 1e-8)
+    cols = [vp(p + (k << 50), p + (k << 50) + (1 << 48)) for k in range(1, 5)]
+    for n in (2 ** 34 - 1023, 2 ** 34, 2 ** 40):
+        assert L.coat_adamw_step_multi(2, cols[0], 1, cols[1], 1, cols[2], cols[3], None, (ctypes.c_int64 * 2)(8, n), hyper, 1, None, None) == -2
