@@ -15,7 +15,7 @@ extern "C" const char* coat_status_string(int status) {
         case COAT_EDTYPE: return "unsupported dtype combination";
         case COAT_EQGROUP: return "Only Support 128 per-group quantization currently";
         case COAT_EALIGN: return "tensor base address is not aligned (16 bytes, or the element's size where the entry point asks for no more)";
-        case COAT_EOVERLAP: return "a tensor that is written shares memory with another tensor of the launch";
+        case COAT_EOVERLAP: return "a tensor that is written shares memory with another tensor of the call";
         default: return status > 0 ? hipGetErrorString((hipError_t)status) : "unknown coat status";
     }
 }

@@ -12,7 +12,8 @@
 // launch, nothing that a captured graph would have to keep alive.
 #include <math.h>
 
-#include <algorithm>
+#include <memory>
+#include <new>
 
 #include "coat_host.h"
 #include "elem_io.h"
@@ -190,23 +191,6 @@ static bool opt_dtype(int dt) { return dt == COAT_F32 || dt == COAT_BF16 || dt =
 static bool elem_aligned(const void* p, int dt) { return ((uintptr_t)p & (dt == COAT_F32 ? 3u : 1u)) == 0; }
 static int64_t norm_chunks(int64_t numel) { return (numel + kNormChunk - 1) / kNormChunk; }
 
-// Whether a tensor that is written shares memory with another tensor of a launch (a block would then read what another has
-// stepped already).  `spans`: begin, end and whether it is written; sorted here.
-struct Span {
-    uintptr_t begin, end;
-    bool written;
-};
-static bool overlap(Span* spans, int n) {
-    std::sort(spans, spans + n, [](const Span& a, const Span& b) { return a.begin < b.begin; });
-    uintptr_t end_any = 0, end_written = 0;
-    for (int i = 0; i < n; i++) {
-        if (spans[i].begin < (spans[i].written ? end_any : end_written)) return true;
-        if (spans[i].end > end_any) end_any = spans[i].end;
-        if (spans[i].written && spans[i].end > end_written) end_written = spans[i].end;
-    }
-    return false;
-}
-
 extern "C" int coat_grad_norm_partials(int count, const int64_t* numel) {
     if (count < 0 || (count > 0 && !numel)) return COAT_EINVAL;
     int64_t total = 0;
@@ -275,22 +259,26 @@ extern "C" int coat_adamw_step_multi(int count, void* const* params, int p_dtype
             !elem_aligned(exp_avg_sq[i], COAT_F32) || (masters && !elem_aligned(masters[i], COAT_F32)))
             return COAT_EALIGN;
     }
-    const int checked = coat_for_each_launch(count, numel, kStepChunk, kStepMax, kStepBlocks, [&](int first, int last, int64_t) {
-        Span spans[5 * kStepMax];
-        int n = 0;
-        for (int i = first; i < last; i++) {
-            const uintptr_t p = (uintptr_t)params[i], g = (uintptr_t)grads[i], m = (uintptr_t)exp_avg[i], v = (uintptr_t)exp_avg_sq[i];
-            const size_t size = (size_t)numel[i];
-            if (size == 0) continue;
-            spans[n++] = {p, p + size * (p_dtype == COAT_F32 ? 4 : 2), true};
-            spans[n++] = {g, g + size * (g_dtype == COAT_F32 ? 4 : 2), false};
-            spans[n++] = {m, m + size * 4, true};
-            spans[n++] = {v, v + size * 4, true};
-            if (masters) spans[n++] = {(uintptr_t)masters[i], (uintptr_t)masters[i] + size * 4, true};
-        }
-        return overlap(spans, n) ? COAT_EOVERLAP : COAT_OK;
-    });
-    if (checked != COAT_OK) return checked;
+    // over all launches: a later one would read what an earlier one has stepped
+    CoatSpan few[5 * kStepMax];
+    std::unique_ptr<CoatSpan[]> many;
+    if (count > kStepMax) {
+        many.reset(new (std::nothrow) CoatSpan[5 * (size_t)count]);
+        if (!many) return (int)hipErrorOutOfMemory;
+    }
+    CoatSpan* spans = many ? many.get() : few;
+    size_t n = 0;
+    for (int i = 0; i < count; i++) {
+        const uintptr_t p = (uintptr_t)params[i], g = (uintptr_t)grads[i], m = (uintptr_t)exp_avg[i], v = (uintptr_t)exp_avg_sq[i];
+        const size_t size = (size_t)numel[i];
+        if (size == 0) continue;
+        spans[n++] = {p, p + size * (p_dtype == COAT_F32 ? 4 : 2), true};
+        spans[n++] = {g, g + size * (g_dtype == COAT_F32 ? 4 : 2), false};
+        spans[n++] = {m, m + size * 4, true};
+        spans[n++] = {v, v + size * 4, true};
+        if (masters) spans[n++] = {(uintptr_t)masters[i], (uintptr_t)masters[i] + size * 4, true};
+    }
+    if (coat_overlap(spans, n)) return COAT_EOVERLAP;
     // hyperparameters in double, rounded once: 1 - beta2 of a beta2 that was already rounded to fp32 is off by 1e-5 at 0.999
     const double beta1 = hyper[0], beta2 = hyper[1];
     Hyper32 H;

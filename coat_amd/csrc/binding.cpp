@@ -18,7 +18,6 @@
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
-#include <algorithm>
 #include <vector>
 
 #include "../../include/coat_hip.h"
@@ -400,22 +399,14 @@ PyObject* adamw_step_multi(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK_VALUE(step >= 1 && step <= INT32_MAX, who, ": invalid step ", step);
     TORCH_CHECK(!scale || (scale->scalar_type() == at::kFloat && scale->numel() == 1 && scale->device() == device), who,
                 ": grad_scale must be one fp32 element on the parameters' device");
-    if (count > 76) {  // more than one launch: the library compares the tensors of each
-        std::vector<void*> written;
-        for (int c : {0, 2, 3, 4})
-            if (c < columns)
-                for (Py_ssize_t i = 0; i < count; i++)
-                    if (numel[i]) written.push_back(address[c][i]);
-        std::sort(written.begin(), written.end());
-        TORCH_CHECK(std::adjacent_find(written.begin(), written.end()) == written.end(), who, ": a tensor that is stepped is given twice");
-    }
     double hyper[5];
     for (int i = 0; i < 5; i++) hyper[i] = real(a[5 + i]);
     const c10::DeviceGuard guard(device);
-    check(lib.coat_adamw_step_multi((int)count, address[0].data(), p_dtype, address[1].data(), g_dtype, (float**)address[2].data(),
-                                    (float**)address[3].data(), masters ? (float**)address[4].data() : nullptr, numel.data(), hyper, (int)step,
-                                    scale ? (const float*)scale->data_ptr() : nullptr, stream_of(params[0])),
-          who);
+    const int status = lib.coat_adamw_step_multi((int)count, address[0].data(), p_dtype, address[1].data(), g_dtype, (float**)address[2].data(),
+                                                 (float**)address[3].data(), masters ? (float**)address[4].data() : nullptr, numel.data(), hyper,
+                                                 (int)step, scale ? (const float*)scale->data_ptr() : nullptr, stream_of(params[0]));
+    TORCH_CHECK(status != COAT_EOVERLAP, who, ": a tensor that is stepped is given twice, or shares memory with another tensor of the call");
+    check(status, who);
     for (Py_ssize_t i = 0; i < count; i++)  // written behind autograd's back: graphs that saved them must notice
         if (!params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
     Py_RETURN_NONE;

@@ -2,6 +2,8 @@
 #pragma once
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "../../include/coat_hip.h"
 
 // Blocks of `threads` that a launch takes in one dimension: HIP has fewer than 2^32 threads there.
@@ -29,4 +31,20 @@ static int coat_for_each_launch(int count, const int64_t* numel, int64_t chunk, 
         if (const int rc = fn(first, i, chunks)) return rc;
     }
     return COAT_OK;
+}
+
+// Whether a tensor that is written shares memory with another tensor.  The spans are sorted here.
+struct CoatSpan {
+    uintptr_t begin, end;
+    bool written;
+};
+static inline bool coat_overlap(CoatSpan* spans, size_t n) {
+    std::sort(spans, spans + n, [](const CoatSpan& a, const CoatSpan& b) { return a.begin < b.begin; });
+    uintptr_t end_any = 0, end_written = 0;
+    for (size_t i = 0; i < n; i++) {
+        if (spans[i].begin < (spans[i].written ? end_any : end_written)) return true;
+        if (spans[i].end > end_any) end_any = spans[i].end;
+        if (spans[i].written && spans[i].end > end_written) end_written = spans[i].end;
+    }
+    return false;
 }

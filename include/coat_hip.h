@@ -30,7 +30,7 @@ enum coat_status {
     COAT_EDTYPE = -3,   /* dtype combination not supported */
     COAT_EQGROUP = -4,  /* optimizer group size other than 128 (fp8_adamw_expand_cuda_kernel.cu:221) */
     COAT_EALIGN = -5,   /* a tensor base address is not aligned as the entry point asks (16 bytes where it says nothing else) */
-    COAT_EOVERLAP = -6  /* a tensor that is written shares memory with another tensor of the launch */
+    COAT_EOVERLAP = -6  /* a tensor that is written shares memory with another tensor of the call */
 };
 
 enum coat_dtype { COAT_F32 = 0, COAT_BF16 = 1, COAT_F16 = 2 };
@@ -435,7 +435,7 @@ int coat_grad_norm_multi(int count, const void* const* grads, const int* dtypes,
  * parameter receiving their rounding.  hyper: host array of five doubles: beta1, beta2 (both in [0, 1)), lr, weight decay,
  * eps.  grad_scale: NULL, or one fp32 in device memory that the gradients are multiplied by (out[1] above).  Host arrays are
  * read before the call returns; addresses need the element's own alignment only; a tensor that is written may share no memory with another
- * tensor (COAT_EOVERLAP where two of one launch do); empty ones are skipped; everything is checked before the first launch. */
+ * tensor of the call (COAT_EOVERLAP); empty ones are skipped; everything is checked before the first launch. */
 int coat_adamw_step_multi(int count, void* const* params, int p_dtype, const void* const* grads, int g_dtype, float* const* exp_avg,
                           float* const* exp_avg_sq, float* const* masters, const int64_t* numel, const double* hyper, int step,
                           const float* grad_scale, void* stream);

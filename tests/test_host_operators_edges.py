@@ -310,3 +310,29 @@ def test_steps_of_tensors_that_no_launch_takes_are_refused_before_the_first():
     cols = [vp(p + (k << 50), p + (k << 50) + (1 << 48)) for k in range(1, 5)]
     for n in (2 ** 34 - 1023, 2 ** 34, 2 ** 40):
         assert L.coat_adamw_step_multi(2, cols[0], 1, cols[1], 1, cols[2], cols[3], None, (ctypes.c_int64 * 2)(8, n), hyper, 1, None, None) == -2
+
+
+@pytest.mark.parametrize("count", [77, 153, 200])
+def test_shared_memory_is_found_over_all_launches_of_a_step(count):
+    """Each pair below lies in two launches; nothing is launched."""
+    import ctypes
+
+    from coat_amd import _hip
+    L, vp, base = _hip.lib(), ctypes.c_void_p * count, 1 << 40
+    numel, hyper = (ctypes.c_int64 * count)(*[100] * count), (ctypes.c_double * 5)(0.9, 0.95, 1e-3, 0.1, 1e-8)
+    cols = [[base + (k << 30) + 400 * i for i in range(count)] for k in range(5)]  # 100 fp32 elements from each
+
+    def status(change, p_dtype=0, masters=False):
+        c = [list(col) for col in cols]
+        for (col, i), at in change.items():
+            c[col][i] = at
+        a = [vp(*col) for col in c]
+        return L.coat_adamw_step_multi(count, a[0], p_dtype, a[1], p_dtype, a[2], a[3], a[4] if masters else None, numel, hyper, 1, None, None)
+
+    last = count - 1
+    assert status({(0, last): cols[0][0]}) == -6                                # a parameter twice
+    assert status({(0, last): cols[0][0] + 396}) == -6                          # its last element
+    assert status({(1, last): cols[0][0] + 4}) == -6                            # a gradient inside an earlier parameter
+    assert status({(1, 0): cols[3][last]}) == -6                                # a later moment
+    assert status({(2, last): cols[3][0] - 396}) == -6                          # a moment into another one
+    assert status({(4, last): cols[2][0] + 200}, p_dtype=1, masters=True) == -6  # a master into a moment
