@@ -15,6 +15,7 @@
 
 #include "coat_host.h"
 #include "elem_io.h"
+#include "tensor_list.h"
 
 namespace coat {
 
@@ -45,7 +46,9 @@ __device__ __forceinline__ uint32_t div_magic(uint32_t n, uint32_t d, uint32_t m
 template <int DT, bool ADJ, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rope_axes(RopeArgs A) {
     __shared__ float2 cs[kRopeSlots];
-    const int64_t first = (int64_t)blockIdx.x * A.per_block;
+    // rows of blocks, as many to a row as a launch takes in one dimension: only the last row can reach past the tokens
+    const int64_t first = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * A.per_block;
+    if (first >= A.tokens) return;
     const int here = (int)(A.tokens - first < A.per_block ? A.tokens - first : A.per_block);
     // a job is one 8-element piece: of the first halves together with the same piece of the second halves, of adjacent pairs,
     // or of the rest behind the pairs
@@ -169,7 +172,8 @@ extern "C" int coat_rope_axes(const void* q, void* q_out, int64_t q_sb, int64_t 
     A.per_block = per;
     const int64_t blocks = (A.tokens + per - 1) / per;
     if (blocks > 0x7fffffffll) return COAT_ESHAPE;
-    const dim3 grid((unsigned)blocks);
+    constexpr int64_t kRow = coat_max_blocks(256);
+    const dim3 grid((unsigned)(blocks < kRow ? blocks : kRow), (unsigned)((blocks + kRow - 1) / kRow));
     hipStream_t st = (hipStream_t)stream;
 #define ROPE(DT)                                                                                                    \
     if (adjacent && whole) hipLaunchKernelGGL((k_rope_axes<DT, true, true>), grid, dim3(256), 0, st, A);             \

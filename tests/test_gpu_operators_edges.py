@@ -91,3 +91,17 @@ def test_a_plan_may_be_dropped_while_another_stream_still_reads_its_tables(dev):
     torch.cuda.synchronize()
     assert torch.equal(out, want) and len(other) == 400
     assert torch.allclose(q.grad, q, rtol=1e-5, atol=1e-5)  # turned there and back
+
+
+def test_more_tokens_than_a_launch_takes_blocks_in_a_row(dev):
+    """2^24 + 5000 tokens whose 520 pairs leave one token to a block; three tokens of a time are compared with their own calls."""
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes_forward
+    S, D = (1 << 24) + 5000, 1040
+    plan = RotaryAxes(D, (200, 320))
+    base = randn(dev, 1, 1, 7, 1, D, dtype=torch.bfloat16)
+    q = torch.as_strided(base, (1, S, 1, D), (7 * D, 0, D, 1))  # the same token everywhere: no 35 GB of input
+    pos = torch.arange(S, device=dev).expand(2, 1, S)
+    out = rotary_axes_forward(q, None, pos, plan)[0]
+    for at in (0, 5, (1 << 24) - 3, (1 << 24) + 2000, S - 3):
+        assert torch.equal(out[:, at:at + 3], rotary_axes_forward(q[:, :3], None, pos[:, :, at:at + 3], plan)[0]), at
+    assert torch.isfinite(out.view(-1)[::997]).all()
