@@ -13,6 +13,7 @@
 
 #include "coat_host.h"
 #include "elem_io.h"
+#include "tensor_list.h"
 
 namespace coat {
 
@@ -383,14 +384,14 @@ __global__ __launch_bounds__(256) void k_ln_bwd_wb_long(const void* __restrict__
 // ------------------------------------------------------------------------------------------------ dw, db from partial rows
 // 32 columns a block (one 128-byte line of each partial row); 32 slices of threads take the rows in turn, eight loads in flight
 // each (one load at a time took 15 us more at 512 x 4096); slice sums are added in slice order.  blockIdx.y: 0 = the first pair
-// given, 1 = the second.
+// given, 1 = the second; blockIdx.z: rows of blocks, as many to a row as a launch takes in one dimension.
 constexpr int kSumCols = 32, kSumSlices = 32;
 __global__ __launch_bounds__(kSumCols* kSumSlices) void k_ln_sum_partials(const float* __restrict__ pw, void* __restrict__ dw,
                                                                          const float* __restrict__ pb, void* __restrict__ db, int dt,
                                                                          int64_t rows, int64_t N) {
     __shared__ float red[kSumSlices][kSumCols];
     const int col = threadIdx.x % kSumCols, slice = threadIdx.x / kSumCols;
-    const int64_t c = (int64_t)blockIdx.x * kSumCols + col;
+    const int64_t c = ((int64_t)blockIdx.z * gridDim.x + blockIdx.x) * kSumCols + col;
     const float* p = blockIdx.y == 0 && dw ? pw : pb;
     void* out = blockIdx.y == 0 && dw ? dw : db;
     float s = 0.0f;
@@ -542,8 +543,10 @@ static int ln_backward(const void* dy, int64_t dy_pitch, const void* x, int64_t 
     }
     if (dw || db) {
         const int64_t rows = M > 0 ? n_partial : 0;  // no rows: the sums are zeros
-        hipLaunchKernelGGL(k_ln_sum_partials, dim3((unsigned)((N + kSumCols - 1) / kSumCols), dw && db ? 2 : 1), dim3(kSumCols * kSumSlices), 0,
-                           st, pw, dw, pb, db, wb_dtype, rows, N);
+        constexpr int64_t kRow = coat_max_blocks(kSumCols * kSumSlices);
+        const int64_t blocks = (N + kSumCols - 1) / kSumCols;
+        const dim3 grid((unsigned)(blocks < kRow ? blocks : kRow), dw && db ? 2 : 1, (unsigned)((blocks + kRow - 1) / kRow));
+        hipLaunchKernelGGL(k_ln_sum_partials, grid, dim3(kSumCols * kSumSlices), 0, st, pw, dw, pb, db, wb_dtype, rows, N);
         return coat_launch_status();
     }
     return COAT_OK;

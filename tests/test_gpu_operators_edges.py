@@ -105,3 +105,19 @@ def test_more_tokens_than_a_launch_takes_blocks_in_a_row(dev):
     for at in (0, 5, (1 << 24) - 3, (1 << 24) + 2000, S - 3):
         assert torch.equal(out[:, at:at + 3], rotary_axes_forward(q[:, :3], None, pos[:, :, at:at + 3], plan)[0]), at
     assert torch.isfinite(out.view(-1)[::997]).all()
+
+
+# ------------------------------------------------------------------------------------------------ LayerNorm
+def test_parameter_gradients_of_more_columns_than_a_launch_takes_blocks_in_a_row(dev):
+    """One row of 2^27 + 100 columns: each gradient is one product, or dy itself, with the roundings of the separate torch operations."""
+    from coat_amd.activation.norm import layer_norm_backward, layer_norm_forward
+    N = (1 << 27) + 100
+    x, dy = (torch.randn(1, N, generator=torch.Generator(dev).manual_seed(s), device=dev) for s in (1, 2))
+    w = torch.ones(N, device=dev)
+    _, mean, rstd = layer_norm_forward(x, w)
+    assert abs(mean.item()) < 1e-3 and abs(rstd.item() - 1) < 1e-3
+    dx, dw, db = layer_norm_backward(dy, x, mean, rstd, w)
+    h = (x - mean) * rstd
+    assert torch.equal(db, dy[0]) and torch.equal(dw, (dy * h)[0]) and torch.isfinite(dx).all()
+    only = layer_norm_backward(dy, x, mean, rstd, w, False, x_grad=False)
+    assert torch.equal(only[1], dw) and only[0] is only[2] is None
