@@ -226,7 +226,7 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (wanted) {
         parts = lib.coat_layer_norm_partials(M, N);
         if (parts < 0) check(parts, who);
-        if (parts > 1 || N > 16384) partial = at::empty({wanted, parts, N}, x.options().dtype(at::kFloat));  // one block needs none
+        if (parts > 1 || N > COAT_LAYER_NORM_ROW) partial = at::empty({wanted, parts, N}, x.options().dtype(at::kFloat));  // one block needs none
     }
     int64_t x_pitch, dy_pitch;
     const at::Tensor xr = rows(x, N, x_pitch), gr = rows(dy, N, dy_pitch);

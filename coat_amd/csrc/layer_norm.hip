@@ -431,7 +431,7 @@ struct LnShape {
 static LnShape ln_shape(int64_t N, bool sums) {
     if (N <= 512) return {256, N <= 64 ? 32 : N <= 128 ? 16 : N <= 256 ? 8 : 4};
     if (N <= 8192) return {(int)((N + 511) / 512) * 64, 1};
-    if (N <= 16384) return {sums ? (int)((N + 2047) / 2048) * 64 : (int)((N + 1023) / 1024) * 64, 1};
+    if (N <= COAT_LAYER_NORM_ROW) return {sums ? (int)((N + 2047) / 2048) * 64 : (int)((N + 1023) / 1024) * 64, 1};
     return {0, 1};
 }
 // Calls f(L, C, RAGGED) (as integral constants) for that form.
@@ -445,6 +445,7 @@ template <bool SUMS, typename F> static void ln_form(int64_t N, F f) {
     else if (N <= 512) { FORM(64, 1); }
     else if (N <= 8192) { FORM(kBlock, 1); }
     else { FORM(kBlock, (SUMS ? 4 : 2)); }
+    static_assert(COAT_LAYER_NORM_ROW == form_threads(kBlock, 4) * 4 * 8 && COAT_LAYER_NORM_ROW == form_threads(kBlock, 2) * 2 * 8, "longest rows");
 #undef FORM
 }
 static int64_t ln_rounds(int64_t M, int64_t N) {

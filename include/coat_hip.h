@@ -308,11 +308,13 @@ int coat_rope_axes(const void* q, void* q_out, int64_t q_sb, int64_t q_ss, int64
  * element's own alignment only.  Sums are fp32, the variance is the two-pass one, y is rounded once. */
 int coat_layer_norm_forward(const void* x, int64_t x_pitch, int x_dtype, const void* w, const void* b, int w_dtype, void* y,
                             float* mean, float* rstd, int64_t M, int64_t N, float eps, void* stream);
+/* Rows of up to so many elements are held in registers: one block then writes dw and db itself, without a workspace. */
+#define COAT_LAYER_NORM_ROW 16384
 /* The n_partial with which coat_layer_norm_backward is fastest on such a tensor, or a negative status. */
 int coat_layer_norm_partials(int64_t M, int64_t N);
 /* dx (dense, x_dtype), dw and db (w_dtype), each optional (NULL).  dy, x of x_dtype with row pitches (0 = N).  partial: fp32
  * workspace [2, n_partial, N] if both dw and db are wanted, [1, n_partial, N] for one, unused for none; 1 <= n_partial <= 65535
- * blocks (with one, partial may be NULL for N <= 16384) each sum their rows into one partial row, which are then added in a fixed
+ * blocks (with one, partial may be NULL for N <= COAT_LAYER_NORM_ROW) each sum their rows into one partial row, which are then added in a fixed
  * order: the same bits every time for one n_partial.  M = 0 gives zero gradients. */
 int coat_layer_norm_backward(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, int x_dtype, const float* mean,
                              const float* rstd, const void* w, int w_dtype, void* dx, void* dw, void* db, float* partial,

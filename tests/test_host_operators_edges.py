@@ -336,3 +336,18 @@ def test_shared_memory_is_found_over_all_launches_of_a_step(count):
     assert status({(1, 0): cols[3][last]}) == -6                                # a later moment
     assert status({(2, last): cols[3][0] - 396}) == -6                          # a moment into another one
     assert status({(4, last): cols[2][0] + 200}, p_dtype=1, masters=True) == -6  # a master into a moment
+
+
+def test_rows_that_are_not_held_in_registers_need_their_workspace():
+    import ctypes
+    import os
+    import re
+
+    from coat_amd import _hip
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    longest = int(re.search(r"#define COAT_LAYER_NORM_ROW (\d+)", open(os.path.join(root, "include", "coat_hip.h")).read()).group(1))
+    keep = ctypes.create_string_buffer(64)
+    p = (ctypes.addressof(keep) + 15) & ~15
+    L = _hip.lib()
+    assert L.coat_layer_norm_partials(1, longest) == L.coat_layer_norm_partials(1, longest + 1) == 1
+    assert L.coat_layer_norm_backward(p, 0, p, 0, 0, p, p, p, 0, p, p, p, None, 1, 1, longest + 1, None) == -1
