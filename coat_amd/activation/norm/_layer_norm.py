@@ -15,7 +15,8 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5):
 
 def layer_norm_backward(dy, x, mean, rstd, weight=None, bias_grad=True, *, x_grad=True, weight_grad=True):
     """Returns ``(dx, dw, db)`` from the forward's x, mean, rstd and weight: dx in x's dtype, dw and db in the weight's; without a
-    weight, or where the gradient is not asked for, None.  dw and db are summed in fp32 in a fixed order."""
+    weight, or where the gradient is not asked for, None.  dw and db are summed in fp32 in a fixed order; each
+    gradient has the same bits whichever others are asked for."""
     return _hip.native().layer_norm_backward(dy, x, mean, rstd, weight, x_grad, weight_grad, bias_grad)
 
 

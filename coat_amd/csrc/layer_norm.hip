@@ -49,6 +49,17 @@ template <int L> __device__ __forceinline__ float row_sum(float v, float* red) {
     __syncthreads();
     return cluster_sum<16>(red[threadIdx.x & 15]);
 }
+// Wave sums of four values, each with the additions of cluster_sum<64>, in three exchanges between 16-lane rows instead of eight:
+// row 0 returns the sum of a0, row 1 of a1, row 2 of b0, row 3 of b1.
+__device__ __forceinline__ float four_wave_sums(float a0, float a1, float b0, float b1) {
+    const bool odd = threadIdx.x & 16, upper = threadIdx.x & 32;
+    a0 = cluster_sum<16>(a0);
+    a1 = cluster_sum<16>(a1);
+    b0 = cluster_sum<16>(b0);
+    b1 = cluster_sum<16>(b1);
+    const float a = (odd ? a1 : a0) + lane_xor_f32(odd ? a0 : a1, 16), b = (odd ? b1 : b0) + lane_xor_f32(odd ? b0 : b1, 16);
+    return (upper ? b : a) + lane_xor_f32(upper ? a : b, 32);
+}
 template <int DT, int L, int C, bool RAGGED>
 __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __restrict__ x, int64_t x_pitch, const void* __restrict__ w,
                                                                  const void* __restrict__ b, int w_dt, void* __restrict__ y,
@@ -139,6 +150,9 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
                                                                  float* __restrict__ pw, float* __restrict__ pb, int64_t M, int N) {
     constexpr int R = form_rows(L);
     constexpr bool kShared = SUMS && R > 1;  // several rows of the block share a column: summed through LDS at the end
+    // Rows of four pieces a lane keep two sums of two pieces each, in the places of the waves that hold those pieces where dx alone is
+    // wanted (two pieces a lane, twice the waves): dx has the same bits with and without the parameters' gradients.
+    constexpr int H = L == kBlock && C == 4 ? 2 : 1;
     constexpr bool kLean = C * (DT == kF32 ? 2 : 1) * (RAGGED ? 2 : 1) >= 8;  // no registers left for the next row
     __shared__ float red[4][16];
     __shared__ float cols[kShared ? R : 1][kShared ? L * C * 8 : 1];
@@ -178,7 +192,9 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
     }
     for (int64_t i = 0; i < rounds; i++, row += step) {
         if (kLean) load(row);
-        float h[C][8], t[C][8], st = 0.0f, sth = 0.0f;
+        float h[C][8], t[C][8], st[H], sth[H];
+#pragma unroll
+        for (int k = 0; k < H; k++) st[k] = sth[k] = 0.0f;
 #pragma unroll
         for (int k = 0; k < C; k++) {
             raw8_to_f32<DT>(rx[k], h[k]);
@@ -192,8 +208,8 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
                 }
                 t[k][j] *= wv[k][j];  // zeros past the row: they add nothing to any sum
                 const float own = !RAGGED || own_element((k * lanes + l) * 8, N, j) ? t[k][j] : 0.0f;
-                st += own;
-                sth = fmaf(own, h[k][j], sth);
+                st[k % H] += own;
+                sth[k % H] = fmaf(own, h[k][j], sth[k % H]);
             }
         }
         const float rs = rstd;
@@ -201,15 +217,21 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_bwd(const void* __res
         if (dx) {
             float mt, mth;
             if (L != kBlock) {
-                mt = row_sum<L>(st, nullptr) * inv_n;
-                mth = row_sum<L>(sth, nullptr) * inv_n;
+                mt = row_sum<L>(st[0], nullptr) * inv_n;
+                mth = row_sum<L>(sth[0], nullptr) * inv_n;
             } else {  // both sums behind one barrier; the buffers alternate from row to row
-                st = cluster_sum<64>(st);
-                sth = cluster_sum<64>(sth);
                 float *ra = red[2 * (i & 1)], *rb = red[2 * (i & 1) + 1];
-                if ((threadIdx.x & 63) == 0) {
-                    ra[threadIdx.x >> 6] = st;
-                    rb[threadIdx.x >> 6] = sth;
+                if (H == 2) {
+                    const float s = four_wave_sums(st[0], st[H - 1], sth[0], sth[H - 1]);
+                    float* to = threadIdx.x & 32 ? rb : ra;
+                    if ((threadIdx.x & 15) == 0) to[(threadIdx.x + (threadIdx.x & 16 ? lanes : 0)) >> 6] = s;
+                } else {
+                    st[0] = cluster_sum<64>(st[0]);
+                    sth[0] = cluster_sum<64>(sth[0]);
+                    if ((threadIdx.x & 63) == 0) {
+                        ra[threadIdx.x >> 6] = st[0];
+                        rb[threadIdx.x >> 6] = sth[0];
+                    }
                 }
                 __syncthreads();
                 mt = cluster_sum<16>(ra[threadIdx.x & 15]) * inv_n;
@@ -518,7 +540,8 @@ static int ln_backward(const void* dy, int64_t dy_pitch, const void* x, int64_t 
                        int64_t M, int64_t N, hipStream_t st) {
     if (n_partial > ln_rounds(M, N)) n_partial = (int)ln_rounds(M, N);
     const bool sums = dw || db;
-    const LnShape shape = ln_shape(N, sums);
+    LnShape shape = ln_shape(N, sums);
+    if (!sums && N > 8192 && shape.threads) shape.threads = 2 * ln_shape(N, true).threads;  // the same halves of a row as with the sums
     if (M > 0 && shape.threads) {
 #define BACKWARD(SUMS, BLOCKS)                                                                                                           \
     ln_form<SUMS>(N, [&](auto lanes, auto pieces, auto ragged) {                                                                         \

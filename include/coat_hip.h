@@ -315,7 +315,7 @@ int coat_layer_norm_partials(int64_t M, int64_t N);
 /* dx (dense, x_dtype), dw and db (w_dtype), each optional (NULL).  dy, x of x_dtype with row pitches (0 = N).  partial: fp32
  * workspace [2, n_partial, N] if both dw and db are wanted, [1, n_partial, N] for one, unused for none; 1 <= n_partial <= 65535
  * blocks (with one, partial may be NULL for N <= COAT_LAYER_NORM_ROW) each sum their rows into one partial row, which are then added in a fixed
- * order: the same bits every time for one n_partial.  M = 0 gives zero gradients. */
+ * order: the same bits every time for one n_partial, and dx the same whatever else is wanted.  M = 0 gives zero gradients. */
 int coat_layer_norm_backward(const void* dy, int64_t dy_pitch, const void* x, int64_t x_pitch, int x_dtype, const float* mean,
                              const float* rstd, const void* w, int w_dtype, void* dx, void* dw, void* db, float* partial,
                              int n_partial, int64_t M, int64_t N, void* stream);

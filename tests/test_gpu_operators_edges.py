@@ -121,3 +121,15 @@ def test_parameter_gradients_of_more_columns_than_a_launch_takes_blocks_in_a_row
     assert torch.equal(db, dy[0]) and torch.equal(dw, (dy * h)[0]) and torch.isfinite(dx).all()
     only = layer_norm_backward(dy, x, mean, rstd, w, False, x_grad=False)
     assert torch.equal(only[1], dw) and only[0] is only[2] is None
+
+
+@pytest.mark.parametrize("M,N", [(3, 8193), (20, 8200), (5, 10239), (7, 10241), (9, 12288), (40, 13712), (300, 14337), (2, 16384)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_frozen_parameters_do_not_change_the_bits_of_dx(dev, M, N, dtype):
+    """Rows that are held in four pieces a lane with the sums of the parameters' gradients, and in two without."""
+    from coat_amd.activation.norm import layer_norm_backward, layer_norm_forward
+    x, dy, w = randn(dev, 1, M, N, dtype=dtype), randn(dev, 2, M, N, dtype=dtype), 1 + randn(dev, 3, N, scale=0.2)
+    _, mean, rstd = layer_norm_forward(x, w)
+    want = layer_norm_backward(dy, x, mean, rstd, w)[0]
+    for weight, bias in ((False, False), (True, False), (False, True)):
+        assert torch.equal(layer_norm_backward(dy, x, mean, rstd, w, bias, weight_grad=weight)[0], want), (weight, bias)
