@@ -40,6 +40,6 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """``torch.nn.functional.layer_norm`` over the last dimension, with reverse-mode autograd, as one kernel forward and one (and the
     reduction of the parameters' gradients) backward.  Forward-mode derivatives are refused (NotImplementedError);
     ``torch.jit.trace`` records the call as one step."""
-    if torch.jit.is_tracing() or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if torch._C._get_tracing_state() or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return _LayerNorm.apply(x, weight, bias, eps)
     return layer_norm_forward(x, weight, bias, eps)[0]

@@ -14,6 +14,7 @@
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -239,11 +240,11 @@ PyObject* layer_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ------------------------------------------------------------------------------------------------ rotary
-// (q, k, positions, turns, axis, head_dim, axes, pairs, adjacent, inverse) -> (q, k)
+// (q, k, positions, turns, axis, head_dim, axes, pairs, adjacent, inverse, stream of the tables) -> (q, k)
 PyObject* rotary_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     const char* who = "rotary_axes";
-    arguments(who, n, 10);
+    arguments(who, n, 11);
     const at::Tensor *q = tensor_or_none(a[0], who, "q"), *k = tensor_or_none(a[1], who, "k");
     at::Tensor pos = tensor(a[2], who, "position_ids");
     const at::Tensor &turns = tensor(a[3], who, "turns"), &axis = tensor(a[4], who, "axis");
@@ -271,6 +272,8 @@ PyObject* rotary_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::DeviceGuard guard(first.device());
     if (pos.scalar_type() != at::kLong) pos = pos.to(at::kLong);
     if (pos.size(1) != B || pos.size(2) != S) pos = pos.expand({axes, B, S});
+    void *const stream = stream_of(first), *const home = PyLong_AsVoidPtr(a[10]);
+    if (!home && PyErr_Occurred()) throw python_error();
     at::Tensor in[2], out[2];
     int64_t strides[2][3] = {};
     int heads[2] = {};
@@ -286,8 +289,13 @@ PyObject* rotary_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check(lib.coat_rope_axes(data(in[0]), data(out[0]), strides[0][0], strides[0][1], strides[0][2], heads[0], data(in[1]), data(out[1]),
                              strides[1][0], strides[1][1], strides[1][2], heads[1], dt, (const int64_t*)pos.data_ptr(), pos.stride(0),
                              pos.stride(1), pos.stride(2), (int)axes, (const double*)turns.data_ptr(), (const int32_t*)axis.data_ptr(), (int)pairs,
-                             (int)D, truth(a[8]), truth(a[9]), B, S, stream_of(first)),
+                             (int)D, truth(a[8]), truth(a[9]), B, S, stream),
           who);
+    if (stream != home) {  // the caller cannot see the tables: kept from reuse until this stream has read them, should their plan be dropped
+        const c10::Stream current = c10::impl::VirtualGuardImpl(first.device().type()).getStream(first.device());
+        turns.record_stream(current);
+        axis.record_stream(current);
+    }
     return tuple({out[0], out[1]});
     END_HANDLE_TH_ERRORS
 }

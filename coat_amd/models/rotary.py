@@ -36,7 +36,7 @@ class RotaryAxes:
         self._start_tables()
 
     def _start_tables(self):
-        self._tables, self._home = {}, {}  # by device: the tables, and the stream whose order their memory follows
+        self._tables, self._home = {}, {}  # by device: the tables, and the handle of the stream whose order their memory follows
         if torch.cuda.is_initialized():
             self.tables(torch.device("cuda", torch.cuda.current_device()))
 
@@ -53,16 +53,8 @@ class RotaryAxes:
         if device not in self._tables:
             turns = torch.tensor([f / (2.0 * math.pi) for f in self._freq], dtype=torch.float64, device=device)
             self._tables[device] = turns, torch.tensor(self._axis, dtype=torch.int32, device=device)
-            self._home[device] = _hip.raw_stream(device.index) if device.type == "cuda" else None
+            self._home[device] = _hip.raw_stream(device.index) if device.type == "cuda" else 0
         return self._tables[device]
-
-    def _use(self, device):
-        """``tables``, kept from reuse until what is queued on the current stream has read them: the caller cannot see these tensors."""
-        tables = self.tables(device)
-        if device.type == "cuda" and _hip.raw_stream(device.index) != self._home[device]:
-            for t in tables:
-                t.record_stream(torch.cuda.current_stream(device))
-        return tables
 
     def cos_sin(self, position_ids, dtype):
         """cos / sin [B, S, head_dim] from torch operations on any device, for heads that turn whole in the (j, j + P) layout;
@@ -81,8 +73,10 @@ def _rotate(q, k, position_ids, plan, inverse):
     first = k if q is None else q
     if first is None:
         raise ValueError("rotary_axes: neither q nor k given")
-    turns, axis = plan._use(first.device)
-    return _hip.native().rotary_axes(q, k, position_ids, turns, axis, plan.head_dim, len(plan.sections), plan.turning, plan.pairs, inverse)
+    device = first.device
+    turns, axis = plan.tables(device)
+    return _hip.native().rotary_axes(q, k, position_ids, turns, axis, plan.head_dim, len(plan.sections), plan.turning, plan.pairs, inverse,
+                                     plan._home[device])
 
 
 def rotary_axes_forward(q, k, position_ids, plan):
@@ -118,6 +112,6 @@ class _RotaryAxes(torch.autograd.Function):
 def rotary_axes(q, k, position_ids, plan):
     """``rotary_axes_forward`` with reverse-mode autograd.  Forward-mode derivatives are refused (NotImplementedError);
     ``torch.jit.trace`` records the call as one step."""
-    if torch.jit.is_tracing() or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+    if torch._C._get_tracing_state() or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
         return _RotaryAxes.apply(q, k, position_ids, plan)
     return rotary_axes_forward(q, k, position_ids, plan)

@@ -80,6 +80,7 @@ def test_a_plan_may_be_dropped_while_another_stream_still_reads_its_tables(dev):
     work, side = randn(dev, 2, 4096, 4096), torch.cuda.Stream()
     torch.cuda.synchronize()
     plan = RotaryAxes(128, (16, 24, 24))
+    addresses = {t.data_ptr() for t in plan.tables(q.device)}
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         for _ in range(20):
@@ -88,8 +89,9 @@ def test_a_plan_may_be_dropped_while_another_stream_still_reads_its_tables(dev):
         out.backward(want.detach(), retain_graph=False)
     del plan
     other = [torch.full((64,), 7.5, dtype=torch.float64, device=dev) for _ in range(200)] + [torch.full((64,), 1, dtype=torch.int32, device=dev) for _ in range(200)]
+    assert not side.query() and not addresses & {t.data_ptr() for t in other}  # not handed out again while that work is queued
     torch.cuda.synchronize()
-    assert torch.equal(out, want) and len(other) == 400
+    assert torch.equal(out, want)
     assert torch.allclose(q.grad, q, rtol=1e-5, atol=1e-5)  # turned there and back
 
 

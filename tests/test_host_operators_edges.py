@@ -12,7 +12,7 @@ def binding_calls(x):
     turns, axis = torch.zeros(4, dtype=torch.float64), torch.zeros(4, dtype=torch.int32)
     return {"forward": lambda: native.layer_norm_forward(x, None, None, 1e-5),
             "backward": lambda: native.layer_norm_backward(x, x, stat, stat, w, True, True, True),
-            "rotary": lambda: native.rotary_axes(x.view(1, 4, 1, 8), None, torch.zeros(1, 1, 4, dtype=torch.int64), turns, axis, 8, 1, 4, False, False),
+            "rotary": lambda: native.rotary_axes(x.view(1, 4, 1, 8), None, torch.zeros(1, 1, 4, dtype=torch.int64), turns, axis, 8, 1, 4, False, False, 0),
             "norm": lambda: native.grad_norm_multi([stat, x], 1.0),
             "step": lambda: native.adamw_step_multi([stat, x], [stat, x], [stat, x], [stat, x], None, *HYPER, None)}
 
@@ -35,7 +35,6 @@ def test_autograd_wrappers_refuse_tangents_with_and_without_requires_grad():
     from coat_amd.activation.norm import layer_norm
     from coat_amd.models.rotary import RotaryAxes, rotary_axes
     plan, pos = RotaryAxes(8, (2, 2)), torch.zeros(2, 1, 4, dtype=torch.int64)
-    plan.tables = lambda device: (torch.zeros(4, dtype=torch.float64), torch.zeros(4, dtype=torch.int32))
     x = torch.randn(1, 4, 1, 8)
     with fwAD.dual_level():
         with pytest.raises(NotImplementedError):
@@ -117,33 +116,7 @@ def test_tables_that_are_not_a_plans_are_refused():
     for bad in ((turns.float(), axis), (turns, axis.long()), (turns[:3], axis), (turns, axis[:3]), (torch.zeros(8, dtype=torch.float64)[::2], axis),
                 (turns, torch.zeros(8, dtype=torch.int32)[::2])):
         with pytest.raises(ValueError, match="tables"):
-            _hip.native().rotary_axes(q, None, pos, *bad, 8, 2, 4, False, False)
-
-
-def test_tables_used_on_another_stream_than_their_own_are_recorded_there(monkeypatch):
-    """The caller of a plan cannot do that: the memory of a dropped plan would be reused under a kernel that still reads it."""
-    from coat_amd import _hip
-    from coat_amd.models.rotary import RotaryAxes
-
-    class Table:
-        def __init__(self):
-            self.recorded = []
-
-        def record_stream(self, s):
-            self.recorded.append(s)
-
-    current, there = [7], torch.device("cuda", 0)
-    monkeypatch.setattr(_hip, "raw_stream", lambda index: current[0])
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: (device, current[0]))
-    plan = RotaryAxes(32, (6, 10))
-    made = []
-    monkeypatch.setattr(torch, "tensor", lambda *a, **kw: made.append(Table()) or made[-1])
-    assert plan._use(there) == tuple(made) and not any(t.recorded for t in made)
-    current[0] = 9
-    plan._use(there)
-    current[0] = 7
-    plan._use(there)
-    assert [t.recorded for t in made] == [[(there, 9)], [(there, 9)]]
+            _hip.native().rotary_axes(q, None, pos, *bad, 8, 2, 4, False, False, 0)
 
 
 # ------------------------------------------------------------------------------------------------ CoatAdamW
