@@ -135,3 +135,24 @@ def test_frozen_parameters_do_not_change_the_bits_of_dx(dev, M, N, dtype):
     want = layer_norm_backward(dy, x, mean, rstd, w)[0]
     for weight, bias in ((False, False), (True, False), (False, True)):
         assert torch.equal(layer_norm_backward(dy, x, mean, rstd, w, bias, weight_grad=weight)[0], want), (weight, bias)
+
+
+# ------------------------------------------------------------------------------------------------ rotary in fp32
+def test_angles_of_fp32_heads_lose_nothing_to_the_rounded_argument(dev):
+    """Heads (1, 0) return cosine and sine themselves.  Bound on how far the angle they stand for is off, in the mean square: two
+    roundings of at most 2^-25 each (the library's result and its correction), uniformly distributed, the library's taken one and a
+    half times as large: sqrt(1 + 1.5^2) 2^-25 / sqrt(3) = 3.1e-8 radians.  An argument rounded to fp32 is off by up to 2^-26 of a turn
+    where it is a quarter turn or more: 5.4e-8 in the mean square by itself."""
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes_backward, rotary_axes_forward
+    plan, S = RotaryAxes(128, (30, 34), theta=500.0), 20000
+    q = torch.zeros(1, S, 1, 128, device=dev)
+    q[..., :64] = 1.0
+    pos = torch.randint(0, 1 << 20, (2, 1, S), generator=torch.Generator().manual_seed(1)).to(dev)
+    freq = torch.tensor([500.0 ** -(j / 64) for j in range(64)], dtype=torch.float64, device=dev)
+    ang = pos[[0] * 30 + [1] * 34].permute(1, 2, 0).double()[:, :, None] * freq
+    for f, sign in ((rotary_axes_forward, 1.0), (rotary_axes_backward, -1.0)):
+        out = f(q, None, pos, plan)[0].double()
+        off = out[..., 64:] * sign * ang.cos() - out[..., :64] * ang.sin()
+        far = ang.cos() < 0  # at least a quarter turn from a whole one
+        assert off[far].square().mean().sqrt() <= 3.25 ** 0.5 * 2.0 ** -25 / 3 ** 0.5, off[far].square().mean().sqrt()
+        assert off.square().mean().sqrt() <= 3.25 ** 0.5 * 2.0 ** -25 / 3 ** 0.5, off.square().mean().sqrt()
