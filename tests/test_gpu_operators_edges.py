@@ -137,6 +137,27 @@ def test_frozen_parameters_do_not_change_the_bits_of_dx(dev, M, N, dtype):
         assert torch.equal(layer_norm_backward(dy, x, mean, rstd, w, bias, weight_grad=weight)[0], want), (weight, bias)
 
 
+@pytest.mark.parametrize("M,N", [(400, 100), (400, 500), (400, 1000), (400, 4096), (400, 5000), (300, 12000), (300, 20000), (200, 40001)])
+def test_rows_far_from_zero_keep_their_mean_to_the_last_bits(dev, M, N):
+    """fp32 rows around m = 1000 with a spread of about 1.  In the mean square over the rows, with u = 2^-24, an error at most as large as
+    the sum it belongs to and uniformly distributed: the additions of a tree take (1 + 1/2 + 1/4 ...) / 3 <= 2/3 of (u m)^2, 16 wave sums
+    one after the other (rows beyond 16384) 1.95 of it, the product 1/3, a rounded 1/N at most 1 in every row alike (a division has
+    none): at most 1.52 u m, with a tenth more for the sample 1.7.  The deviations are off by that, and by at most 20 roundings of
+    themselves (8 squares a piece, two pieces and 13 operations, half of it after the root; then the last three)."""
+    from coat_amd.activation.norm import layer_norm_forward
+    x = randn(dev, N, M, N) * (0.5 + torch.rand(M, 1, generator=torch.Generator().manual_seed(1)).to(dev)) + 1000.0
+    y, mean, rstd = layer_norm_forward(x, None, None, 1e-5)
+    xd, u = x.double(), 2.0 ** -24
+    m = xd.mean(1)
+    d = xd - m[:, None]
+    r = (d.square().mean(1) + 1e-5).rsqrt()
+    rms = lambda t: t.square().mean().sqrt()  # noqa: E731
+    assert rms(mean.double() - m) <= 1.7 * u * rms(m), rms(mean.double() - m) / (u * rms(m))
+    off = y.double() / r[:, None] - d
+    assert rms(off) <= u * (1.7 * rms(m) + 20 * rms(d)), rms(off) / (u * (1.7 * rms(m) + 20 * rms(d)))
+    assert ((rstd.double() / r - 1).abs() <= (20 + N / 1024) * u + (4 * u * m * r) ** 2).all()
+
+
 # ------------------------------------------------------------------------------------------------ rotary in fp32
 def test_angles_of_fp32_heads_lose_nothing_to_the_rounded_argument(dev):
     """Heads (1, 0) return cosine and sine themselves.  Bound on how far the angle they stand for is off, in the mean square: two
