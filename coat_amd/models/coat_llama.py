@@ -536,7 +536,9 @@ class LlamaSdpaAttentionWithoutLinear(nn.Module):
                 q, k = q.transpose(1, 2), k.transpose(1, 2)
             else:  # evaluation on the CPU, in torch operations like the rest of the layer there
                 cos, sin = self.rotary_axes.cos_sin(position_ids, q.dtype)
-                q, k = apply_rotary_pos_emb(q.transpose(1, 2), k.transpose(1, 2), cos, sin)
+                q, k, n = q.transpose(1, 2), k.transpose(1, 2), cos.shape[-1]
+                turned = apply_rotary_pos_emb(q[..., :n], k[..., :n], cos, sin)
+                q, k = turned if n == self.head_dim else (torch.cat((t, x[..., n:]), -1) for t, x in zip(turned, (q, k)))
         elif position_embeddings is None and query_states.is_cuda and query_states.dtype == torch.bfloat16:
             # one fused kernel per tensor and direction instead of mul / neg / cat / add passes
             max_pos = getattr(self.config, "max_position_embeddings", None)

@@ -57,10 +57,10 @@ class RotaryAxes:
         return self._tables[device]
 
     def cos_sin(self, position_ids, dtype):
-        """cos / sin [B, S, head_dim] from torch operations on any device, for heads that turn whole in the (j, j + P) layout;
+        """cos / sin [B, S, 2 P] of the first 2 P elements of a head from torch operations on any device, in the (j, j + P) layout;
         position_ids [axes, B, S]."""
-        if self.pairs or 2 * self.turning != self.head_dim:
-            raise ValueError("RotaryAxes.cos_sin: only for heads that turn whole, in the (j, j + P) layout")
+        if self.pairs:
+            raise ValueError("RotaryAxes.cos_sin: only for the (j, j + P) layout")
         if position_ids.dim() != 3 or position_ids.shape[0] != len(self.sections):
             raise ValueError(f"RotaryAxes: expected position_ids of shape [{len(self.sections)}, batch, seq], got {list(position_ids.shape)}")
         freq = torch.tensor(self._freq, dtype=torch.float64, device=position_ids.device)

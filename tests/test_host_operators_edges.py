@@ -324,3 +324,22 @@ def test_rows_that_are_not_held_in_registers_need_their_workspace():
     L = _hip.lib()
     assert L.coat_layer_norm_partials(1, longest) == L.coat_layer_norm_partials(1, longest + 1) == 1
     assert L.coat_layer_norm_backward(p, 0, p, 0, 0, p, p, p, 0, p, p, p, None, 1, 1, longest + 1, None) == -1
+
+
+# ------------------------------------------------------------------------------------------------ the decoder layer
+def test_attention_on_the_cpu_turns_a_part_of_the_head_as_the_gpu_does():
+    from coat_amd.models.coat_llama import CoatLlamaConfig, LlamaSdpaAttentionWithoutLinear, apply_rotary_pos_emb
+    g = torch.Generator().manual_seed(0)
+    config = CoatLlamaConfig(hidden_size=64, num_attention_heads=2, num_key_value_heads=1, rotary_sections=(3, 2, 6))  # 22 of 32 elements
+    module = LlamaSdpaAttentionWithoutLinear(config).eval()
+    q, k, v = (torch.randn(1, 7, n, generator=g) for n in (64, 32, 32))
+    pos = torch.randint(0, 50, (3, 1, 7), generator=g)
+    out = module(q, k, v, position_ids=pos)[0]
+    freq = 10000.0 ** -(torch.arange(11, dtype=torch.float64) / 11)
+    ang = torch.cat((pos[0, 0, :, None] * freq[:3], pos[1, 0, :, None] * freq[3:5], pos[2, 0, :, None] * freq[5:]), -1)
+    ang = torch.cat((ang, ang), -1)[None]
+    heads = [t.view(1, 7, -1, 32).transpose(1, 2).double().expand(1, 2, 7, 32) for t in (q, k, v)]
+    turned = apply_rotary_pos_emb(heads[0][..., :22], heads[1][..., :22], ang.cos(), ang.sin())
+    rq, rk = (torch.cat((t, h[..., 22:]), -1) for t, h in zip(turned, heads))
+    s = (rq @ rk.transpose(2, 3) / 32 ** 0.5).masked_fill(torch.triu(torch.ones(7, 7, dtype=torch.bool), 1), float("-inf")).softmax(-1)
+    assert torch.allclose(out.double(), (s @ heads[2]).transpose(1, 2).reshape(1, 7, 64), rtol=0, atol=1e-5)
