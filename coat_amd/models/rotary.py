@@ -52,7 +52,10 @@ class RotaryAxes:
         """(turns a position fp64 [P], axis int32 [P]) on ``device``."""
         if device not in self._tables:
             turns = torch.tensor([f / (2.0 * math.pi) for f in self._freq], dtype=torch.float64, device=device)
-            self._tables[device] = turns, torch.tensor(self._axis, dtype=torch.int32, device=device)
+            axis = torch.tensor(self._axis, dtype=torch.int32, device=device)
+            if type(turns) is not torch.Tensor:  # of a mode that computes without memory: not for later calls
+                return turns, axis
+            self._tables[device] = turns, axis
             self._home[device] = _hip.raw_stream(device.index) if device.type == "cuda" else 0
         return self._tables[device]
 
@@ -76,7 +79,7 @@ def _rotate(q, k, position_ids, plan, inverse):
     device = first.device
     turns, axis = plan.tables(device)
     return _hip.native().rotary_axes(q, k, position_ids, turns, axis, plan.head_dim, len(plan.sections), plan.turning, plan.pairs, inverse,
-                                     plan._home[device])
+                                     plan._home.get(device, 0))
 
 
 def rotary_axes_forward(q, k, position_ids, plan):

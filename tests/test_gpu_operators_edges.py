@@ -109,6 +109,26 @@ def test_more_tokens_than_a_launch_takes_blocks_in_a_row(dev):
     assert torch.isfinite(out.view(-1)[::997]).all()
 
 
+def test_plans_made_and_dropped_around_a_capture(dev):
+    from coat_amd.models.rotary import RotaryAxes, rotary_axes_forward
+    q, pos = randn(dev, 1, 1, 9, 2, 128), torch.arange(9, device=dev).expand(3, 1, 9)
+    plan, other = RotaryAxes(128, (16, 24, 24)), RotaryAxes(128, (16, 24, 24), theta=500.0)
+    rotary_axes_forward(q, None, pos, other)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rotary_axes_forward(q, None, pos, plan)[0]
+        del other
+    for k in range(3):
+        q.copy_(randn(dev, 5 + k, 1, 9, 2, 128))
+        graph.replay()
+        assert torch.equal(out, rotary_axes_forward(q, None, pos, plan)[0])
+    del graph, plan
+    fresh = [torch.zeros(64, dtype=torch.float64, device=dev) for _ in range(50)]
+    torch.cuda.synchronize()
+    want = rotary_axes_forward(q, None, pos, RotaryAxes(128, (16, 24, 24)))[0]
+    assert torch.equal(out, want) and not any(t.any() for t in fresh)
+
+
 # ------------------------------------------------------------------------------------------------ LayerNorm
 def test_parameter_gradients_of_more_columns_than_a_launch_takes_blocks_in_a_row(dev):
     """One row of 2^27 + 100 columns: each gradient is one product, or dy itself, with the roundings of the separate torch operations."""

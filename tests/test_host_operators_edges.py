@@ -119,6 +119,18 @@ def test_tables_that_are_not_a_plans_are_refused():
             _hip.native().rotary_axes(q, None, pos, *bad, 8, 2, 4, False, False, 0)
 
 
+def test_plans_keep_no_tables_of_tensors_without_memory():
+    """Tables made while a model runs on fake tensors would be refused by every later call."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from coat_amd.models.rotary import RotaryAxes
+    plan, cpu = RotaryAxes(32, (6, 10)), torch.device("cpu")
+    with FakeTensorMode():
+        assert plan.tables(cpu)[0].shape == (16,)
+    turns, axis = plan.tables(cpu)
+    assert type(turns) is type(axis) is torch.Tensor and turns[0].item() > 0.1
+
+
 # ------------------------------------------------------------------------------------------------ CoatAdamW
 class Calls:
     """The kernels' Python entries replaced: what the optimizer hands them."""
