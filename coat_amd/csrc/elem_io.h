@@ -1,7 +1,8 @@
 // Wide loads and stores of 16- and 32-bit elements at any element alignment, for the kernels that take row slices, odd row
 // lengths and tensors laid out one after the other without padding.  The hardware's global loads and stores need no more
 // than the element's own alignment (the code objects run in unaligned access mode), so a 16-byte access that crosses a line
-// costs one more line, not a loop over elements: only the last, incomplete piece of a row goes element by element.
+// costs one more line, not a loop over elements.  A row that ends inside a piece takes its last eight elements as the last piece
+// (piece_begin); only rows of fewer than eight, and the ends that load8 / load4 are given, go element by element.
 #pragma once
 #include "coat_device.h"
 

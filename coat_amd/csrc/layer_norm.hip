@@ -138,8 +138,11 @@ __global__ __launch_bounds__(form_threads(L, C)) void k_ln_fwd(const void* __res
     }
 }
 
-// x and dy are not needed again after this kernel: streaming loads ([262144, 128] bf16: 42 -> 39 us with the sums; with the caches
-// full of another kernel's writes 44 against 68; in the forward, whose x the backward reads, 24 -> 26).
+// x and dy are not needed again after this kernel: streaming loads.  In a training step dy has just been written and x, of the forward,
+// has left the caches: [262144, 128] bf16 40 us against 45 with ordinary loads, [8192, 4096] bf16 43 against 50, [8192, 1024] fp32 29
+// against 30; with neither in the caches 45 against 70.  Ordinary loads are better off only where both were just written and fit
+// (fp32 [8192, 1024] 25 against 28; bf16 as above 40 against 40), which a forward in between rules out.  Streaming x alone: 39, 46, 29.  In the
+// forward, whose x the backward reads, streaming costs 24 -> 26.
 // dx, and with SUMS the sums for dw and db (either may be NULL): one partial row per block, in pw / pb, or, if there is one block
 // only, dw and db themselves.
 template <int DT, int L, int C, bool RAGGED, bool SUMS>
