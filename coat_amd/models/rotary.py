@@ -55,8 +55,8 @@ class RotaryAxes:
             axis = torch.tensor(self._axis, dtype=torch.int32, device=device)
             if type(turns) is not torch.Tensor:  # of a mode that computes without memory: not for later calls
                 return turns, axis
-            self._tables[device] = turns, axis
             self._home[device] = _hip.raw_stream(device.index) if device.type == "cuda" else 0
+            self._tables[device] = turns, axis  # last: another thread that finds the tables finds their stream
         return self._tables[device]
 
     def cos_sin(self, position_ids, dtype):

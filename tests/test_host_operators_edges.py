@@ -131,6 +131,20 @@ def test_plans_keep_no_tables_of_tensors_without_memory():
     assert type(turns) is type(axis) is torch.Tensor and turns[0].item() > 0.1
 
 
+def test_tables_appear_after_their_stream():
+    """A thread that finds the tables of another one's first call must find the stream they belong to."""
+    from coat_amd.models.rotary import RotaryAxes
+
+    class Order(dict):
+        def __setitem__(self, key, value):
+            assert key in plan._home
+            super().__setitem__(key, value)
+
+    plan = RotaryAxes(32, (6, 10))
+    plan._tables = Order()
+    plan.tables(torch.device("cpu"))
+
+
 # ------------------------------------------------------------------------------------------------ CoatAdamW
 class Calls:
     """The kernels' Python entries replaced: what the optimizer hands them."""
